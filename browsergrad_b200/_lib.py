@@ -8,6 +8,9 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from typing import Sequence
+
+from .errors import KernelError
 
 MAX_RANK = 8
 MAX_STEP_INPUTS = 8
@@ -59,6 +62,61 @@ class ProfileEntry(C.Structure):
     _fields_ = [("name", C.c_char * 64), ("ms", C.c_float), ("launches", C.c_int32)]
 
 
+class HeadView(C.Structure):
+    """Where the heads of a tensor lie in a bridge buffer: head ``h`` of row ``s`` of batch ``b`` is the run of values from
+    element ``offset + b * stride[0] + s * stride[1] + h * stride[2]`` (``bg_head_view``)."""
+
+    _fields_ = [("handle", C.c_int64), ("offset", C.c_int64), ("stride", C.c_int64 * 3)]
+
+    def __init__(self, handle: int, strides: Sequence[int], offset: int = 0) -> None:
+        super().__init__(int(handle), int(offset), (C.c_int64 * 3)(*[int(v) for v in strides]))
+
+    @classmethod
+    def heads_first(cls, handle: int, rows: int, heads: int, dim: int) -> "HeadView":
+        """A dense ``[batch, heads, rows, dim]`` buffer: a cache, or what ``flash_attention`` takes."""
+        return cls(handle, (heads * rows * dim, dim, rows * dim))
+
+    @classmethod
+    def rows_first(cls, handle: int, rows: int, heads: int, dim: int, first: int = 0) -> "HeadView":
+        """Heads from ``first`` on of a dense ``[batch, rows, heads, dim]`` buffer: what a projection leaves; ``heads``
+        counts all heads of a row (q, k and v of a packed projection)."""
+        return cls(handle, (rows * heads * dim, heads * dim, dim), first * dim)
+
+
+ROTARY_SCALING = {"none": 0, "linear": 1, "ramp": 2}
+
+
+class RotarySpec(C.Structure):
+    """Which values of a head are turned by their position and how fast (``bg_rotary_spec``): the first ``dim`` values, as
+    pairs (j, j + dim / 2) or, ``interleaved``, (2j, 2j + 1), by position * base^(-2j / dim), times ``magnitude``.
+    ``scaling``: "none"; "linear", frequencies divided by ``factor``; "ramp", the same for pairs that turn fewer than
+    ``low`` times within ``original_length``, none for those that turn more than ``high`` times, linear in between."""
+
+    _fields_ = [("dim", C.c_int32), ("interleaved", C.c_int32), ("scaling", C.c_int32), ("reserved", C.c_int32),
+                ("base", C.c_double), ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("original_length", C.c_double), ("magnitude", C.c_double)]
+
+    def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, scaling: str = "none", factor: float = 1.0,
+                 low: float = 1.0, high: float = 4.0, original_length: float = 0.0, magnitude: float = 1.0) -> None:
+        if scaling not in ROTARY_SCALING:
+            raise KernelError(f"CUDA bridge: rotary: unknown scaling {scaling!r}", 1)
+        super().__init__(int(dim), int(bool(interleaved)), ROTARY_SCALING[scaling], 0, float(base), float(factor), float(low),
+                         float(high), float(original_length), float(magnitude))
+
+
+class AttentionRules(C.Structure):
+    _fields_ = [("scale", C.c_double), ("softcap", C.c_double), ("causal", C.c_int32), ("reserved", C.c_int32),
+                ("slopes", C.c_int64), ("documents", C.c_int64), ("prefixes", C.c_int64), ("lengths", C.c_int64),
+                ("starts", C.c_int64)]
+
+
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double), ("top_k", C.c_int64),
+                ("temperatures", C.c_int64), ("top_ks", C.c_int64), ("top_ps", C.c_int64), ("min_ps", C.c_int64)]
+
+
+_VIEW = C.POINTER(HeadView)
+
 # name -> (restype, argtypes); every symbol include/bgcuda.h declares
 SIGNATURES = {
     "bg_abi_version": (C.c_int, []),
@@ -93,6 +151,14 @@ SIGNATURES = {
                                            C.c_int64, C.c_void_p, C.c_char_p, C.c_size_t]),
     "bg_selftest_wait_timeout": (C.c_int, [C.c_void_p, C.c_int64]),
     "bg_alloc": (C.c_int, [C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.c_int, C.POINTER(C.c_int64)]),
+    "bg_rotary": (C.c_int, [C.c_void_p, _VIEW, C.POINTER(RotarySpec)] + [C.c_int64] * 4 +
+                  [C.c_int, C.c_int64, C.c_int64, C.c_int, _VIEW, C.POINTER(C.c_int64)]),
+    "bg_rotary_append": (C.c_int, [C.c_void_p] + [_VIEW] * 5 + [C.POINTER(RotarySpec)] + [C.c_int64] * 6 +
+                         [C.c_int, C.c_int64, C.c_int64, C.c_int64, _VIEW, C.POINTER(C.c_int64)]),
+    "bg_decoder_attention": (C.c_int, [C.c_void_p] + [_VIEW] * 3 + [C.c_int64] * 6 +
+                             [C.c_int, C.POINTER(AttentionRules), _VIEW, C.POINTER(C.c_int64)]),
+    "bg_sample_tokens": (C.c_int, [C.c_void_p] + [C.c_int64] * 4 + [C.c_int, C.POINTER(Sampling), C.c_int64, C.c_int64,
+                                                                    C.POINTER(C.c_int64)]),
     "bg_stream": (C.c_void_p, [C.c_void_p]),
     "bg_device_pointer": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(C.c_void_p)]),
 }

@@ -15,11 +15,13 @@ batched; REDUCE has max/min/argmax/any/all; CONST, WHERE, INDEX, CROSS_ENTROPY a
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Any, Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 
 from . import _lib, wire
+from ._lib import HeadView, RotarySpec
 from .errors import KernelError
 
 
@@ -171,6 +173,72 @@ class CudaBridge:
         self._check(self._lib.bg_flash_attention(self._ctx, int(q), int(k), int(v), int(mask or 0), ms, int(b), int(h),
                                                  int(sq), int(sk), int(d), float(scale), self._dt(dtype), C.byref(out)))
         return int(out.value)
+
+    # -- serving operators (no counterpart in the reference bridge; rules in include/bgcuda.h) --------
+    # Views: a handle alone is a dense [batch, heads, rows, dim] buffer, a HeadView any other layout.  Results go into
+    # ``out`` when given, else into a fresh buffer, dense like the operands; the handle is returned either way.
+    @staticmethod
+    def _view(x: Any, heads: int, rows: int, dim: int) -> Any:
+        return C.byref(x if isinstance(x, HeadView) else HeadView.heads_first(x, rows, heads, dim))
+
+    @staticmethod
+    def _out_view(out: Any) -> Any:
+        if out is None:
+            return None
+        if not isinstance(out, HeadView):
+            raise KernelError("CUDA bridge: `out` must be a HeadView", 1)
+        return C.byref(out)
+
+    def rotary(self, x: Any, spec: RotarySpec, b: int, h: int, s: int, d: int, dtype: str, positions: Optional[int] = None,
+               start: int = 0, inverse: bool = False, out: Optional[HeadView] = None) -> int:
+        """``x [b, s, h, d]`` with its heads turned by their positions: ``positions`` (int32 ``[b, s]``), or ``start + s``.
+        ``inverse`` turns back.  ``out`` may be ``x``'s own view."""
+        r = C.c_int64()
+        self._check(self._lib.bg_rotary(self._ctx, self._view(x, h, s, d), C.byref(spec), b, h, s, d, self._dt(dtype), positions or 0,
+                                        start, 1 if inverse else 0, self._out_view(out), C.byref(r)))
+        return r.value
+
+    def rotary_append(self, q: Any, k: Any, v: Any, k_cache: Any, v_cache: Any, spec: RotarySpec, b: int, hq: int, hkv: int,
+                      s: int, capacity: int, d: int, dtype: str, starts: Optional[int] = None, start: int = 0,
+                      counts: Optional[int] = None, out: Optional[HeadView] = None) -> int:
+        """The new rows of a step in one launch: ``q`` turned (the result), ``k`` turned into rows ``starts[b] + s`` (or
+        ``start + s``) of ``k_cache``, ``v`` into the same rows of ``v_cache``; with ``counts`` (int32 ``[b]``) only the
+        first ``counts[b]`` rows of a sequence are stored.  Caches hold ``capacity`` rows."""
+        r = C.c_int64()
+        self._check(self._lib.bg_rotary_append(
+            self._ctx, self._view(q, hq, s, d), self._view(k, hkv, s, d), self._view(v, hkv, s, d), self._view(k_cache, hkv, capacity, d),
+            self._view(v_cache, hkv, capacity, d), C.byref(spec), b, hq, hkv, s, capacity, d, self._dt(dtype), starts or 0, start,
+            counts or 0, self._out_view(out), C.byref(r)))
+        return r.value
+
+    def decoder_attention(self, q: Any, k: Any, v: Any, b: int, hq: int, hkv: int, sq: int, sk: int, d: int, dtype: str,
+                          scale: Optional[float] = None, causal: bool = True, softcap: float = 0.0, slopes: Optional[int] = None,
+                          documents: Optional[int] = None, prefixes: Optional[int] = None, lengths: Optional[int] = None,
+                          starts: Optional[int] = None, out: Optional[HeadView] = None) -> int:
+        """Attention of ``sq`` rows over ``sk`` cached ones, ``hq`` query heads sharing ``hkv`` key heads; ``scale`` is
+        ``1 / sqrt(d)`` unless given.  ``softcap`` caps the scores, ``slopes`` (float32 ``[hq]``) subtracts slope *
+        distance, ``documents`` (int32 ``[b, sk]``, below zero: none), ``prefixes``, ``lengths`` and ``starts`` (int32
+        ``[b]``) say which keys a row sees; a row that sees none is zero."""
+        r = C.c_int64()
+        rules = _lib.AttentionRules(1.0 / math.sqrt(d) if scale is None and d > 0 else scale or 0.0, softcap, 1 if causal else 0, 0, slopes or 0,
+                                    documents or 0, prefixes or 0, lengths or 0, starts or 0)
+        self._check(self._lib.bg_decoder_attention(self._ctx, self._view(q, hq, sq, d), self._view(k, hkv, sk, d),
+                                                   self._view(v, hkv, sk, d), b, hq, hkv, sq, sk, d, self._dt(dtype), C.byref(rules),
+                                                   self._out_view(out), C.byref(r)))
+        return r.value
+
+    def sample_tokens(self, logits: int, uniforms: int, n: int, vocab: int, dtype: str, temperature: float = 1.0, top_k: int = 0,
+                      top_p: float = 1.0, min_p: float = 0.0, temperatures: Optional[int] = None, top_ks: Optional[int] = None,
+                      top_ps: Optional[int] = None, min_ps: Optional[int] = None, probabilities: Optional[int] = None,
+                      out: Optional[int] = None) -> int:
+        """One token (int64 ``[n]``) per row of ``logits [n, vocab]`` from the random numbers ``uniforms`` (float32 ``[n]``
+        in [0, 1)).  Temperature 0 is greedy.  The plural parameters are per-row buffers (float32, ``top_ks`` int32);
+        ``probabilities`` names a float32 ``[n]`` buffer for the tokens' chances."""
+        r = C.c_int64()
+        sampling = _lib.Sampling(temperature, top_p, min_p, top_k, temperatures or 0, top_ks or 0, top_ps or 0, min_ps or 0)
+        self._check(self._lib.bg_sample_tokens(self._ctx, logits, uniforms, n, vocab, self._dt(dtype), C.byref(sampling),
+                                               probabilities or 0, out or 0, C.byref(r)))
+        return r.value
 
     # -- outside the forward path ----------------------------------------------------------
     def _unsupported(self, name: str) -> Any:

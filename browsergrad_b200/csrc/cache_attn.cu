@@ -1,0 +1,58 @@
+// Launch planning of the attention over a cache, and the per-block document ranges it skips keys by.
+#include "cache_attn.cuh"
+
+namespace bg {
+namespace {
+
+// Smallest and largest id of each 128 keys (ids below zero belong to no document).  One warp per block.
+__global__ void doc_ranges_kernel(const int* documents, int b, int sk, int blocks, int2* ranges) {
+  const long long w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (w >= (long long)b * blocks) return;
+  const int batch = (int)(w / blocks), blk = (int)(w % blocks), lane = threadIdx.x & 31;
+  int lo = INT_MAX, hi = -1;
+  for (int i = lane; i < kDocBlock; i += 32) {
+    const int key = blk * kDocBlock + i;
+    const int id = key < sk ? documents[(long long)batch * sk + key] : -1;
+    if (id >= 0) { lo = min(lo, id); hi = max(hi, id); }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) ranges[w] = make_int2(lo, hi);
+}
+
+}  // namespace
+
+cudaError_t launch_doc_ranges(const int* documents, int b, int sk, int2* ranges, cudaStream_t s) {
+  const int blocks = (sk + kDocBlock - 1) / kDocBlock;
+  const long long warps = (long long)b * blocks;
+  doc_ranges_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, s>>>(documents, b, sk, blocks, ranges);
+  return cudaGetLastError();
+}
+
+CacheAttnPlan cache_attention_plan(const DecoderAttention& p, int dtype, int sm_count) {
+  CacheAttnPlan plan;
+  const int rows = p.group * p.sq;
+  plan.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int per_cta = 16 * plan.row_tiles;
+  const long long units = (long long)p.b * p.hkv * ((rows + per_cta - 1) / per_cta);
+  // Keys are split over CTAs only while the sets of rows alone do not fill the SMs, and no finer than 512 keys: a CTA's
+  // start, its join and the reading of its partial result cost about as much as that many keys.
+  long long splits = units >= sm_count ? 1 : sm_count / units;
+  const long long most = (p.sk + 511) / 512;
+  if (splits > most) splits = most;
+  if (splits > cache_attn::kMaxSplits) splits = cache_attn::kMaxSplits;
+  if (splits < 1) splits = 1;
+  plan.splits = (int)splits;
+  plan.partial_bytes = splits > 1 ? units * splits * per_cta * (cache_attn::padded_head(p.d) + 2) * 4 : 0;
+  (void)dtype;
+  return plan;
+}
+
+cudaError_t launch_cache_attention(const DecoderAttention& p, int dtype, const CacheAttnPlan& plan, float* partials, int* counters,
+                                   cudaStream_t s) {
+  if (dtype == BG_BF16) return cache_attn::launch_bf16(p, plan, partials, counters, s);
+  if (dtype == BG_F16) return cache_attn::launch_f16(p, plan, partials, counters, s);
+  return cache_attn::launch_f32(p, plan, partials, counters, s);
+}
+
+}  // namespace bg

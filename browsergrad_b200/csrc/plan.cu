@@ -3536,7 +3536,7 @@ int take_device_status(bg_context* ctx) {
 }
 
 std::string device_status_message(int status_rc) {
-  return status_rc == BG_ERR_INDEX_RANGE ? "run_tensor_plan: gather / scatter / cross_entropy index outside its axis, or scatter indices naming one destination twice"
+  return status_rc == BG_ERR_INDEX_RANGE ? "run_tensor_plan: gather / scatter / cross_entropy index outside its axis, scatter indices naming one destination twice, or a length, count or cache row outside its buffer"
          : status_rc == BG_ERR_DEVICE_TIMEOUT ? "run_tensor_plan: a device-side wait of a tensor-core kernel gave up (status 6)"
                                               : "run_tensor_plan: device-side status " + std::to_string(status_rc);
 }
@@ -3678,6 +3678,11 @@ int run_plan(bg_context* ctx, const bg_plan* plan, const bg_plan_input* inputs, 
   if (out_host) {
     int rc = d2h(ctx, out_host, run.ptr[cp->root_slot], (size_t)cp->root_bytes);
     cleanup(false);
+    if (rc == BG_OK && ctx->status_pending) {
+      // the copy synchronised the stream: what earlier work refused on the device is known now
+      const int st = take_device_status(ctx);
+      if (st != 0) return fail(ctx, st, device_status_message(st) + " (in an earlier plan)");
+    }
     return rc;
   }
   *out_handle = mint_handle(ctx, run.ptr[cp->root_slot], cp->root_bytes, cp->root_dtype, cp->root_shape, cp->root_rank);

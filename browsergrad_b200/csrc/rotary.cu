@@ -1,0 +1,164 @@
+// Rotary positions, alone or together with the append of new keys and values to a cache (sm_100a).
+//
+// A pair (a, b) of a head at position t becomes (a cos w - b sin w, a sin w + b cos w), w = t f_j.  The work is bound by
+// memory: every value is read and written once.  A CTA takes a few consecutive tokens of one sequence with all their
+// heads, so the angles -- which all heads share -- are computed once per token into shared memory and the loop over heads
+// only loads, multiplies and stores, 16 bytes per access, both halves of a pair's vectors in flight together.
+// Angles: t f_j reaches 10^6 radians and more, where 32 bits leave no fraction; the product is formed in 64 bits as turns
+// (f_j / 2 pi comes from the host), its whole part is taken off, and sine and cosine of the fraction are 32-bit.  The
+// rotation is done in 32 bits and rounded once to the stored type.
+// Measured (32771 tokens, 32 heads of 128, bf16): see the table of the design notes.
+#include "serving.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace bg {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 16;
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T)) Vec {
+  T v[VEC];
+};
+
+// One item: the vectors at elements c * VEC of the first half and of the second half of the rotated part.
+template <typename T, int VEC, bool INTER>
+__device__ __forceinline__ void turn_item(Vec<T, VEC>& lo, Vec<T, VEC>& hi, const float2* cs, int c, int half) {
+  if (!INTER) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float2 w = cs[c * VEC + i];
+      const float a = to_f(lo.v[i]), b = to_f(hi.v[i]);
+      lo.v[i] = from_f<T>(a * w.x - b * w.y);
+      hi.v[i] = from_f<T>(a * w.y + b * w.x);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const float2 w = cs[(c * VEC + i) >> 1], z = cs[(half + c * VEC + i) >> 1];
+      const float a = to_f(lo.v[i]), b = to_f(lo.v[i + 1]), e = to_f(hi.v[i]), f = to_f(hi.v[i + 1]);
+      lo.v[i] = from_f<T>(a * w.x - b * w.y);
+      lo.v[i + 1] = from_f<T>(a * w.y + b * w.x);
+      hi.v[i] = from_f<T>(e * z.x - f * z.y);
+      hi.v[i + 1] = from_f<T>(e * z.y + f * z.x);
+    }
+  }
+}
+
+// VEC = 1 handles what vectors cannot: odd sizes, strides or addresses that are not multiples of a vector.  An item is
+// then one pair of values, wherever the layout puts its two members.
+template <typename T, int VEC, bool INTER>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryProblem p, int tokens_per_cta, int tiles) {
+  __shared__ float2 s_cs[kMaxTokens * kRotaryMaxPairs];
+  const int batch = blockIdx.x / tiles;
+  const int s0 = (blockIdx.x % tiles) * tokens_per_cta;
+  const int n_tok = min(tokens_per_cta, p.s - s0);
+  const int half = p.rot >> 1;
+  const int64_t first = p.starts ? (int64_t)p.starts[batch] : p.start;
+  for (int i = threadIdx.x; i < n_tok * half; i += kThreads) {
+    const int tok = i / half, j = i - tok * half;
+    const int64_t at = p.positions ? (int64_t)p.positions[(int64_t)batch * p.s + s0 + tok] : first + s0 + tok;
+    const double turns = (double)at * p.turns[j];
+    const float frac = (float)(turns - rint(turns));
+    float sn, cs;
+    sincospif(2.0f * frac, &sn, &cs);
+    s_cs[i] = make_float2(cs * p.magnitude, sn * p.magnitude);
+  }
+  int64_t count = p.s;
+  if (p.counts) {
+    count = p.counts[batch];
+    if (count < 0 || count > p.s) {
+      if (threadIdx.x == 0) { *p.status.host = BG_ERR_INDEX_RANGE; *p.status.device = BG_ERR_INDEX_RANGE; }
+      count = count < 0 ? 0 : p.s;
+    }
+  }
+  __syncthreads();
+  const int pairs = half / VEC;                 // items of the rotated part (two vectors each)
+  const int rest = (p.d - p.rot) / VEC;         // vectors behind it
+  const int per_head = pairs + rest;
+  int h_total = 0;
+  for (int g = 0; g < p.n_seg; ++g) h_total += p.seg[g].heads;
+  const int items = n_tok * h_total * per_head;
+  using V = Vec<T, VEC>;
+  for (int it = threadIdx.x; it < items; it += kThreads) {
+    const int c = it % per_head;
+    int head = (it / per_head) % h_total;
+    const int tok = it / (per_head * h_total);
+    int g = 0;
+    while (head >= p.seg[g].heads) head -= p.seg[g++].heads;
+    const RotarySegment& sg = p.seg[g];
+    int64_t row_out = s0 + tok;
+    if (sg.cached) {
+      if (s0 + tok >= count) continue;
+      row_out += first;
+      if (row_out < 0 || row_out >= p.capacity) {
+        *p.status.host = BG_ERR_INDEX_RANGE;
+        *p.status.device = BG_ERR_INDEX_RANGE;
+        continue;
+      }
+    }
+    const T* x = reinterpret_cast<const T*>(sg.in.ptr) + batch * sg.in.sb + (int64_t)(s0 + tok) * sg.in.sr + head * sg.in.sh;
+    T* y = reinterpret_cast<T*>(const_cast<void*>(sg.out.ptr)) + batch * sg.out.sb + row_out * sg.out.sr + head * sg.out.sh;
+    if (c < pairs) {
+      const int e0 = VEC == 1 && INTER ? 2 * c : c * VEC;
+      const int e1 = VEC == 1 && INTER ? 2 * c + 1 : half + c * VEC;
+      V lo = *reinterpret_cast<const V*>(x + e0), hi = *reinterpret_cast<const V*>(x + e1);
+      if (sg.turn) turn_item<T, VEC, INTER && VEC != 1>(lo, hi, s_cs + tok * half, c, half);
+      *reinterpret_cast<V*>(y + e0) = lo;
+      *reinterpret_cast<V*>(y + e1) = hi;
+    } else {
+      const int e = p.rot + (c - pairs) * VEC;
+      *reinterpret_cast<V*>(y + e) = *reinterpret_cast<const V*>(x + e);
+    }
+  }
+}
+
+template <typename T, int VEC>
+cudaError_t launch_vec(const RotaryProblem& p, cudaStream_t s) {
+  int heads = 0;
+  for (int g = 0; g < p.n_seg; ++g) heads += p.seg[g].heads;
+  const int per_token = heads * (p.rot / 2 / VEC + (p.d - p.rot) / VEC);
+  // four items a thread: enough loads in flight without emptying the grid
+  int tok = (4 * kThreads + per_token - 1) / per_token;
+  if (tok > kMaxTokens) tok = kMaxTokens;
+  if (tok > p.s) tok = p.s;
+  const int64_t tiles = (p.s + tok - 1) / tok;
+  if (tiles * p.b > 0x7fffffffll) return cudaErrorInvalidValue;
+  const unsigned grid = (unsigned)(tiles * p.b);
+  if (p.interleaved) rotary_kernel<T, VEC, true><<<grid, kThreads, 0, s>>>(p, tok, (int)tiles);
+  else rotary_kernel<T, VEC, false><<<grid, kThreads, 0, s>>>(p, tok, (int)tiles);
+  return cudaGetLastError();
+}
+
+// Whether every access of `vec` elements is aligned to its own size.
+bool vectors_fit(const RotaryProblem& p, int vec, int es) {
+  if ((p.rot / 2) % vec || (p.d - p.rot) % vec) return false;
+  for (int g = 0; g < p.n_seg; ++g)
+    for (const HeadPtr* h : {&p.seg[g].in, &p.seg[g].out})
+      if (reinterpret_cast<uintptr_t>(h->ptr) % (uintptr_t)(vec * es) || h->sb % vec || h->sr % vec || h->sh % vec) return false;
+  return true;
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const RotaryProblem& p, int dtype, cudaStream_t s, int) {
+  const int es = dtype_size(dtype);
+  if (dtype == BG_F32) return vectors_fit(p, 4, es) ? launch_vec<float, 4>(p, s) : launch_vec<float, 1>(p, s);
+  const bool bf = dtype == BG_BF16;
+  if (vectors_fit(p, 8, es)) return bf ? launch_vec<__nv_bfloat16, 8>(p, s) : launch_vec<__half, 8>(p, s);
+  if (vectors_fit(p, 4, es)) return bf ? launch_vec<__nv_bfloat16, 4>(p, s) : launch_vec<__half, 4>(p, s);
+  return bf ? launch_vec<__nv_bfloat16, 1>(p, s) : launch_vec<__half, 1>(p, s);
+}
+
+}  // namespace bg

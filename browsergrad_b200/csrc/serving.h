@@ -1,0 +1,85 @@
+// Internal declarations of the serving operators: rotary positions, attention over a key / value cache, token sampling.
+#pragma once
+
+#include "common.h"
+
+namespace bg {
+
+// A resolved bg_head_view: element strides over batch, row and head; the values of one head are contiguous.
+struct HeadPtr {
+  const void* ptr;
+  int64_t sb, sr, sh;
+};
+// Where a kernel reports refused data: the context's device word, and its pinned host copy (device-visible), so that no
+// copy has to follow the launch.
+struct StatusWords {
+  int* device;
+  int* host;
+};
+
+// ---- rotary.cu ---------------------------------------------------------------------------------------------------
+constexpr int kRotaryMaxPairs = 128;
+struct RotarySegment {
+  HeadPtr in, out;
+  int heads;
+  int turn;        // rotate (else copy)
+  int cached;      // rows go to start + s of the cache, those at or behind counts[b] nowhere
+};
+struct RotaryProblem {
+  RotarySegment seg[3];
+  int n_seg;
+  int b, s, d, rot, interleaved;
+  int64_t capacity;           // rows of the caches
+  int64_t start;
+  const int* starts;          // [b] or null (then `start`)
+  const int* positions;       // [b, s] or null (then start + s)
+  const int* counts;          // [b] or null (then s)
+  float magnitude;
+  double turns[kRotaryMaxPairs];   // full turns per position of each pair, signed by the direction
+  StatusWords status;
+};
+cudaError_t launch_rotary(const RotaryProblem& p, int dtype, cudaStream_t s, int sm_count);
+
+// ---- attention over a cache --------------------------------------------------------------------------------------
+struct DecoderAttention {
+  int b, hq, hkv, group, sq, sk, d;
+  HeadPtr q, k, v, out;       // k, v: heads are the hkv shared ones
+  float scale;
+  float cap;                  // 0: none
+  const float* slopes;        // [hq] or null
+  const int* documents;       // [b, sk] or null
+  const int* prefixes;        // [b] or null
+  const int* lengths;         // [b] or null (then sk)
+  const int* starts;          // [b] or null (then lengths[b] - sq)
+  int causal;
+  const int2* doc_ranges;     // [b, ceil(sk / 128)] smallest and largest id of each 128 keys; set with documents
+  StatusWords status;
+};
+constexpr int kDocBlock = 128;
+cudaError_t launch_doc_ranges(const int* documents, int b, int sk, int2* ranges, cudaStream_t s);
+
+// Key-split kernel (cache_attn.cu): every type and head size up to 256, few rows per key head or many.
+struct CacheAttnPlan {
+  int row_tiles;        // 16-row tiles one CTA works on
+  int splits;           // CTAs that share the keys of one set of rows
+  int64_t partial_bytes;
+};
+CacheAttnPlan cache_attention_plan(const DecoderAttention& p, int dtype, int sm_count);
+cudaError_t launch_cache_attention(const DecoderAttention& p, int dtype, const CacheAttnPlan& plan, float* partials, int* counters,
+                                   cudaStream_t s);
+
+// ---- sample.cu ---------------------------------------------------------------------------------------------------
+struct SampleProblem {
+  const void* logits;
+  int64_t n, vocab;
+  const float* uniforms;
+  const float* temperatures; float temperature;
+  const int* top_ks; int top_k;
+  const float* top_ps; float top_p;
+  const float* min_ps; float min_p;
+  int64_t* tokens;
+  float* probabilities;       // or null
+};
+cudaError_t launch_sample(const SampleProblem& p, int dtype, cudaStream_t s, int sm_count);
+
+}  // namespace bg

@@ -44,7 +44,8 @@ typedef enum bg_status {
   BG_ERR_OOM = 4,             /* device allocation failed                                */
   BG_ERR_UNKNOWN_HANDLE = 5,  /* handle was never minted or already released             */
   BG_ERR_DEVICE_TIMEOUT = 6,  /* a bounded device-side wait ran out                      */
-  BG_ERR_INDEX_RANGE = 7      /* gather / cross-entropy index outside its axis           */
+  BG_ERR_INDEX_RANGE = 7      /* gather / cross-entropy index outside its axis, a length or
+                                 cache row outside its buffer                            */
 } bg_status;
 
 /* dtype names of the IR (packages/browsergrad-jit/src/python/_ir.py:348-353) + bfloat16,
@@ -211,6 +212,85 @@ int bg_cast(bg_context* ctx, bg_handle h, int src_dtype, int dst_dtype, const in
 int bg_flash_attention(bg_context* ctx, bg_handle q, bg_handle k, bg_handle v, bg_handle mask,
                        const int64_t* mask_shape, int64_t b, int64_t h, int64_t sq, int64_t sk,
                        int64_t d, double scale, int dtype, bg_handle* out);
+
+/* -- serving operators (no counterpart in the reference bridge, which has neither positions inside a head nor a key /
+ *    value cache nor a way from logits to a token): one generation step is rotary_append, decoder_attention over the
+ *    cache, the decoder's own layers, and sample_tokens.  Operands are float32, float16 or bfloat16, one type per call.
+ *    Results are written into `out_view` / `out_handle` when one is given (the caller's buffer; it must be none of the
+ *    call's other operands), else into a buffer minted for them.  Index buffers are int32.  A call into a stream that is
+ *    being captured into a graph is refused (BG_ERR_UNSUPPORTED).  Values only the device sees (lengths, counts, cache
+ *    rows) are range-checked there: one outside its range is treated as the nearest legal one, nothing outside a buffer
+ *    is touched, and the next call that synchronises or starts other work returns BG_ERR_INDEX_RANGE. --------------- */
+
+/* Where the heads of a tensor lie in a buffer: head h of row s of batch b is the d consecutive values from element
+ * offset + b * stride[0] + s * stride[1] + h * stride[2].  Any order of the axes, rows of a packed projection, a range of
+ * a cache; strides are not negative and every value lies inside the buffer. */
+typedef struct bg_head_view {
+  bg_handle handle;
+  int64_t offset;
+  int64_t stride[3];
+} bg_head_view;
+
+typedef enum bg_rotary_scaling { BG_ROTARY_PLAIN = 0, BG_ROTARY_LINEAR = 1, BG_ROTARY_RAMP = 2 } bg_rotary_scaling;
+/* The first `dim` values of a head (even, <= 256) are pairs: (2j, 2j + 1) when interleaved, else (j, j + dim / 2); pair j
+ * of a row at position t is turned by t * f_j, f_j = base^(-2j / dim), and multiplied by `magnitude`; the values behind
+ * `dim` are copied.  LINEAR: f_j / factor.  RAMP: f_j * (g + (1 - g) / factor) with g = clamp((original_length * f_j /
+ * 2 pi - low) / (high - low), 0, 1): pairs that turn often within the original length keep their frequency. */
+typedef struct bg_rotary_spec {
+  int32_t dim, interleaved, scaling, reserved;
+  double base, factor, low, high, original_length, magnitude;
+} bg_rotary_spec;
+
+/* x [b, s, h, d] -> out: row s at positions[b, s], or at start + s when positions is 0.  inverse turns backwards, which is
+ * also the gradient with respect to x.  out_view may be x's own view (in place). */
+int bg_rotary(bg_context* ctx, const bg_head_view* x, const bg_rotary_spec* spec, int64_t b, int64_t h, int64_t s, int64_t d,
+              int dtype, bg_handle positions, int64_t start, int inverse, const bg_head_view* out_view, bg_handle* out);
+/* One launch for a step's new rows: row s of sequence b has position starts[b] + s (start + s when starts is 0); q is
+ * turned into the result, k is turned and stored at row starts[b] + s of k_cache [b, capacity, hkv, d], v is stored there
+ * in v_cache.  With counts only the first counts[b] rows of a sequence enter the caches; all other cache rows stay as they
+ * were. */
+int bg_rotary_append(bg_context* ctx, const bg_head_view* q, const bg_head_view* k, const bg_head_view* v, const bg_head_view* k_cache,
+                     const bg_head_view* v_cache, const bg_rotary_spec* spec, int64_t b, int64_t hq, int64_t hkv, int64_t s,
+                     int64_t capacity, int64_t d, int dtype, bg_handle starts, int64_t start, bg_handle counts,
+                     const bg_head_view* out_view, bg_handle* out);
+
+/* Attention of sq query rows over sk key rows, hq query heads in groups that share hkv key heads, d <= 256.
+ * Row i of sequence b stands at position t = starts[b] + i (lengths[b] - sq + i when starts is 0: the rows are the last
+ * ones); the score of key j is s = scale q.k_j, then softcap * tanh(s / softcap) when softcap > 0, then - slopes[h] *
+ * |t - j|.  It is seen when all of these hold:
+ *   j < lengths[b] (sk when lengths is 0);
+ *   not causal, or 0 <= t < lengths[b] and (j <= t or j < prefixes[b]);
+ *   no documents, or documents[b, t] = documents[b, j] >= 0.
+ * out = softmax over the seen keys times v; a row that sees none is zero.  Statistics and sums are 32-bit.  Keys and
+ * values at or behind the length are not used, whatever they hold; those in front of it must be finite. */
+typedef struct bg_attention_rules {
+  double scale, softcap;
+  int32_t causal, reserved;
+  bg_handle slopes;      /* float32 [hq] */
+  bg_handle documents;   /* int32 [b, sk] */
+  bg_handle prefixes;    /* int32 [b]; causal only */
+  bg_handle lengths;     /* int32 [b] */
+  bg_handle starts;      /* int32 [b] */
+} bg_attention_rules;
+int bg_decoder_attention(bg_context* ctx, const bg_head_view* q, const bg_head_view* k, const bg_head_view* v, int64_t b, int64_t hq,
+                         int64_t hkv, int64_t sq, int64_t sk, int64_t d, int dtype, const bg_attention_rules* rules,
+                         const bg_head_view* out_view, bg_handle* out);
+
+/* One token per row of logits [n, vocab], as int64 [n].  Weights are e^((x - max) / temperature); a token is kept when
+ * its rank (largest first, equal ones by index) is below top_k (0: all), when the weights ranked before it sum to less
+ * than top_p of the first top_k (>= 1: all), and when its weight is at least min_p of the largest; the largest is always
+ * kept.  The result is the first kept index whose running sum in index order exceeds uniforms[row] (float32, [0, 1)) of
+ * the kept sum.  Temperature 0 takes the largest, the first of equal ones.  -inf and NaN are never drawn; a row of nothing
+ * else gives -1.  Per-row parameters (float32 / int32 [n]) replace the common ones when given; there a temperature that is
+ * not positive is greedy, a top_k that is not positive and a top_p that is not below 1 keep all.  `probabilities`
+ * (float32 [n], 0 for none) receives the chance of the token among the kept ones (1 when greedy, 0 with token -1). */
+typedef struct bg_sampling {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  bg_handle temperatures, top_ks, top_ps, min_ps;
+} bg_sampling;
+int bg_sample_tokens(bg_context* ctx, bg_handle logits, bg_handle uniforms, int64_t n, int64_t vocab, int dtype,
+                     const bg_sampling* sampling, bg_handle probabilities, bg_handle out_handle, bg_handle* out);
 
 /* -- whole-plan methods: run_tensor_plan[_resident] (_bridge.py:262-289;
  *    realizer.ts:1557-1652).  The *_semantic variants differ only in the shim, which checks
