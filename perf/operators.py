@@ -286,39 +286,41 @@ def _bridge():
     return _BRIDGE
 
 
-class _Window:
-    """A device buffer of the bridge as torch sees it."""
+class _Buffer:
+    """A device buffer of the bridge, as torch sees it; it lives as long as the tensors made of it."""
 
-    def __init__(self, pointer, shape, typestr):
-        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": typestr, "data": (pointer, False), "version": 3}
+    _KIND = {"float32": "<f4", "float16": "<f2", "bfloat16": "<i2", "int32": "<i4", "int64": "<i8"}
+
+    def __init__(self, shape, dtype):
+        self.bridge, self.dtype = _bridge(), dtype
+        self.handle = self.bridge.alloc(shape, dtype)
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": self._KIND[dtype], "version": 3,
+                                         "data": (self.bridge.device_pointer(self.handle), False)}
+
+    def tensor(self):
+        t = torch.as_tensor(self, device="cuda")
+        return t.view(torch.bfloat16) if self.dtype == "bfloat16" else t
+
+    def __del__(self):
+        self.bridge.release(self.handle)
 
 
 class _Device:
     """A case's inputs and outputs in buffers of the bridge, and the call on them."""
 
     def __init__(self, case, tensors):
-        self.bridge, self.case, self.handles = _bridge(), case, []
-        h = {k: self._put(v) for k, v in tensors.items()}
-        self.h, self.views = {k: v[0] for k, v in h.items()}, {k: v[1] for k, v in h.items()}
+        self.bridge, self.case = _bridge(), case
+        buffers = {k: _Buffer(tuple(v.shape), str(v.dtype).replace("torch.", "")) for k, v in tensors.items()}
+        self.h, self.views = {k: v.handle for k, v in buffers.items()}, {k: v.tensor() for k, v in buffers.items()}
         getattr(self, "_setup_" + case["op"])()
+        self.bridge.synchronize()  # the buffers are there
+        for k, v in tensors.items():
+            self.views[k].copy_(v)
         torch.cuda.synchronize()
 
     def _new(self, shape, dtype):
-        handle = self.bridge.alloc(shape, dtype)
-        self.handles.append(handle)
-        self.bridge.synchronize()
-        kind = {"float32": "<f4", "float16": "<f2", "bfloat16": "<i2", "int32": "<i4", "int64": "<i8"}[dtype]
-        t = torch.as_tensor(_Window(self.bridge.device_pointer(handle), shape, kind), device="cuda")
-        return handle, t.view(torch.bfloat16) if dtype == "bfloat16" else t
-
-    def _put(self, tensor):
-        handle, view = self._new(tuple(tensor.shape), str(tensor.dtype).replace("torch.", ""))
-        view.copy_(tensor)
-        return handle, view
-
-    def __del__(self):
-        for handle in self.handles:
-            self.bridge.release(handle)
+        buffer = _Buffer(shape, dtype)
+        return buffer.handle, buffer.tensor()
 
     def _setup_rotary(self):
         from browsergrad_b200 import HeadView, RotarySpec
