@@ -4,20 +4,24 @@
 namespace bg {
 namespace {
 
-// Smallest and largest id of each 128 keys (ids below zero belong to no document).  One warp per block.
+// Smallest and largest id of each 128 keys (ids below zero belong to no document, see DecoderAttention::doc_ranges).
+// One warp per block.
 __global__ void doc_ranges_kernel(const int* documents, int b, int sk, int blocks, int2* ranges) {
   const long long w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
   if (w >= (long long)b * blocks) return;
   const int batch = (int)(w / blocks), blk = (int)(w % blocks), lane = threadIdx.x & 31;
   int lo = INT_MAX, hi = -1;
+  bool none = false;
   for (int i = lane; i < kDocBlock; i += 32) {
     const int key = blk * kDocBlock + i;
     const int id = key < sk ? documents[(long long)batch * sk + key] : -1;
     if (id >= 0) { lo = min(lo, id); hi = max(hi, id); }
+    else none = true;
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
-  if (lane == 0) ranges[w] = make_int2(lo, hi);
+  none = __any_sync(0xffffffffu, none);
+  if (lane == 0) ranges[w] = make_int2(none ? lo | (int)0x80000000 : lo, hi);
 }
 
 }  // namespace

@@ -178,7 +178,7 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
     if (ranges)
       while (t < t_end) {
         const int2 rg = __ldg(ranges + t * KT / kDocBlock);
-        if (rg.x <= doc_max && rg.y >= doc_min) break;
+        if ((rg.x & 0x7fffffff) <= doc_max && rg.y >= doc_min) break;
         t += KG;
       }
     return t;

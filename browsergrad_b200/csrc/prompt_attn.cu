@@ -1,0 +1,676 @@
+// Attention of prompts over a cache, 16-bit operands, head dimensions up to 128 (sm_100a): the rules of cache_attn.cuh on
+// the tensor cores of this generation.
+//
+// A CTA owns 256 consecutive query rows of one head as two tiles of 128 (A, B) that share the key and value tiles in
+// shared memory; while the softmax of one tile runs, the products of the other do.
+//   warp 0       producer (lane 0: Q, then K tiles; lane 1: V tiles; TMA)
+//   warps 1, 2   issue the products of tile A and of tile B: S = Q K^T into tensor memory, O += P V with P read from there
+//   warp 3       clears the value rows of the tile the sequence ends in that lie behind its length: a probability of zero
+//                times what an unwritten cache holds would not be zero
+//   warps 4-7    softmax of tile A, one thread per query row; warps 8-11: of tile B
+// With 64 values a head P has columns of its own in tensor memory, and the scores of the next key tile are computed
+// while a tile's softmax still runs; with 128 values the 512 columns are S and O of both tiles, P takes the place of the
+// scores it was made from, and the next scores wait for P V.  The reference of the exponentials follows the row maximum
+// lazily: O is rescaled when the maximum has grown by more than 2^8.
+// Which keys a row sees is one number, the end of its visible range, and for packed documents the row's id: tiles nobody
+// sees are not loaded, tiles everybody sees are not masked, the rest are masked in tensor memory away from the main path.
+// Bound: 4 D flops a visible pair on the tensor pipe (1024 clocks a tile of 128 x 128 x 128) against one exponential a
+// pair on the MUFU (16 a clock: 1024 clocks).  A cap would add two more MUFU operations; within |s| <= cap, where scores
+// nearly always lie, tanh is an odd polynomial on the FMA pipe instead, two values an instruction.
+// No cluster multicast; every wait is clock-bounded.
+#include "serving.h"
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+#include "attn_common.cuh"
+#include "tc_common.cuh"
+
+namespace bg {
+namespace {
+
+using namespace tc;
+using attn::ex2_approx;
+using attn::fmax3;
+using attn::tma_load_4d;
+
+constexpr int kRows = 128, kKeys = 128, kThreads = 384;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazyLog2 = 8.0f;
+constexpr int kMaxPos = 1 << 30;
+// Registers move from warps 0-3 to the softmax warps: (128 x 72 + 256 x 216) / 384 = 168 a thread, what the CTA is
+// launched with (checked at launch; a request beyond the pool would wait for ever).
+constexpr int kLaunchRegs = 168, kLightRegs = 72, kSoftmaxRegs = 216;
+static_assert(128 * kLightRegs + 256 * kSoftmaxRegs <= kLaunchRegs * kThreads, "setmaxnreg requests exceed the CTA's registers");
+
+template <int D>
+struct Cfg {
+  static constexpr bool Alias = D == 128;                    // P in the columns of S
+  static constexpr int Boxes = D / 64;                       // 128-byte wide boxes of a row
+  static constexpr int BoxBytes = 128 * 128;                 // 128 rows of 64 values
+  static constexpr int TileBytes = Boxes * BoxBytes;
+  static constexpr int Stages = 2;
+  static constexpr int ColS = 0, ColO = 256, ColP = Alias ? 0 : 384, StepP = Alias ? 128 : 64;
+  static constexpr int Smem = 2 * TileBytes + 2 * Stages * TileBytes;
+};
+
+struct PromptParams {
+  DecoderAttention a;
+  uint32_t idesc_qk, idesc_pv;
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float a0, float a1) {
+  if (BF16) { __nv_bfloat162 v = __floats2bfloat162_rn(a0, a1); return *reinterpret_cast<uint32_t*>(&v); }
+  __half2 v = __floats2half2_rn(a0, a1);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+// two values an instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float c, float d, float e, float f) {      // (x, y) = (a c + e, b d + f)
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%6, %7};\n\t"
+      "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d), "f"(e), "f"(f));
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b, float c, float d) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b, float c, float d) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d));
+}
+
+// ---- rare work, out of the main path ----
+
+// Replaces the scores of this thread's row that are not seen by -inf; returns a bit per 32 keys none of which is seen.
+__device__ __noinline__ uint32_t hide_scores(uint32_t t_s, uint4 seen) {
+  uint32_t r[128];
+  tmem_ld32_issue(t_s, r);
+  tmem_ld32_issue(t_s + 32, r + 32);
+  tmem_ld32_issue(t_s + 64, r + 64);
+  tmem_ld32_issue(t_s + 96, r + 96);
+  tmem_ld_wait();
+  const uint32_t w[4] = {seen.x, seen.y, seen.z, seen.w};
+#pragma unroll
+  for (int i = 0; i < 128; ++i)
+    if (!((w[i >> 5] >> (i & 31)) & 1u)) r[i] = __float_as_uint(-CUDART_INF_F);
+  tmem_st32_issue(t_s, r);
+  tmem_st32_issue(t_s + 32, r + 32);
+  tmem_st32_issue(t_s + 64, r + 64);
+  tmem_st32_issue(t_s + 96, r + 96);
+  tmem_st_wait();
+  return (w[0] == 0u ? 1u : 0u) | (w[1] == 0u ? 2u : 0u) | (w[2] == 0u ? 4u : 0u) | (w[3] == 0u ? 8u : 0u);
+}
+// Bits of the keys (of `keys` that exist from docs on) whose document is this lane's.  Each key's id is read once per warp;
+// the rows of a warp belong to few documents, so the words are made per document, by ballots, not per row.
+__device__ __noinline__ uint4 document_bits(const int* docs, int keys, int doc) {
+  const int lane = threadIdx.x & 31;
+  int id[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) id[c] = c * 32 + lane < keys ? __ldg(docs + c * 32 + lane) : -1;
+  uint4 w = make_uint4(0u, 0u, 0u, 0u);
+  uint32_t left = __ballot_sync(0xffffffffu, doc >= 0);
+  while (left) {
+    const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
+    const uint4 v = make_uint4(__ballot_sync(0xffffffffu, id[0] == d), __ballot_sync(0xffffffffu, id[1] == d),
+                               __ballot_sync(0xffffffffu, id[2] == d), __ballot_sync(0xffffffffu, id[3] == d));
+    if (doc == d) w = v;
+    left &= ~__ballot_sync(0xffffffffu, doc == d);
+  }
+  return w;
+}
+template <int D>
+__device__ __noinline__ void rescale_row(uint32_t t_o, float alpha) {
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t r[32];
+    tmem_ld32(t_o + (uint32_t)(c * 32), r);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+    tmem_st32(t_o + (uint32_t)(c * 32), r);
+  }
+}
+
+// Rows [i0, i1] of sequence b: the positions among them that see any key, and how many keys the last of them sees.
+struct Reach {
+  int first, last, keys;       // first > last: none
+};
+__device__ __forceinline__ Reach reach_of(const DecoderAttention& a, int b, int len, int i0, int i1) {
+  const long long start = a.starts ? (long long)a.starts[b] : (long long)len - a.sq;
+  long long p0 = start + i0, p1 = start + i1;
+  if (!a.causal) {
+    p0 = min(max(p0, (long long)-kMaxPos), (long long)kMaxPos);
+    p1 = min(max(p1, (long long)-kMaxPos), (long long)kMaxPos);
+    return Reach{(int)p0, (int)p1, i0 <= i1 ? len : 0};
+  }
+  p0 = max(p0, 0ll);
+  p1 = min(p1, (long long)len - 1);
+  if (i0 > i1 || p0 > p1) return Reach{1, 0, 0};
+  return Reach{(int)p0, (int)p1, (int)min((long long)len, max(p1 + 1, (long long)(a.prefixes ? a.prefixes[b] : 0)))};
+}
+
+template <bool BF16, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                        const __grid_constant__ PromptParams pp) {
+  using C = Cfg<D>;
+  const DecoderAttention& a = pp.a;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* sQ = smem;
+  unsigned char* sK = sQ + 2 * C::TileBytes;
+  unsigned char* sV = sK + C::Stages * C::TileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + C::Stages * C::TileBytes);
+  uint64_t* q_full = bars;                       // [2]
+  uint64_t* k_full = q_full + 2;                 // [Stages]
+  uint64_t* k_empty = k_full + C::Stages;
+  uint64_t* v_full = k_empty + C::Stages;
+  uint64_t* v_empty = v_full + C::Stages;
+  uint64_t* s_full = v_empty + C::Stages;        // [2] the scores of a tile are there
+  uint64_t* s_empty = s_full + 2;                // [2] its softmax warps hold them in registers (unused when P takes their place)
+  uint64_t* p_full = s_empty + 2;                // [2] P is there
+  uint64_t* pv_full = p_full + 2;                // [2] P V has completed
+  uint64_t* v_clean = pv_full + 2;               // the value tile the sequence ends in has been cleared behind it
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(v_clean + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  unsigned char* s_need = reinterpret_cast<unsigned char*>(tmem_holder + 4);     // [2][n_kv]
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int n_bh = a.b * a.hq;
+  const int n_qt = (a.sq + kRows - 1) / kRows, n_pairs = (n_qt + 1) / 2;
+  const int pair = n_pairs - 1 - (int)(blockIdx.x / (unsigned)n_bh);       // the last rows see the most keys: they go first
+  const int bh = (int)(blockIdx.x % (unsigned)n_bh);
+  const int b = bh / a.hq, h = bh % a.hq, hk = h / a.group;
+  const bool has_b = 2 * pair + 1 < n_qt;
+
+  int len = a.sk;
+  if (a.lengths) {
+    len = a.lengths[b];
+    if (len < 0 || len > a.sk) {
+      if (threadIdx.x == 0) { *a.status.host = BG_ERR_INDEX_RANGE; *a.status.device = BG_ERR_INDEX_RANGE; }
+      len = min(max(len, 0), a.sk);
+    }
+  }
+  const int n_kv = (len + kKeys - 1) / kKeys;
+  const int2* ranges = a.documents ? a.doc_ranges + (long long)b * ((a.sk + kDocBlock - 1) / kDocBlock) : nullptr;
+  const int* docs = a.documents ? a.documents + (long long)b * a.sk : nullptr;
+  // which key tiles each query tile needs
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int i0 = (2 * pair + g) * kRows, i1 = min(i0 + kRows, a.sq) - 1;
+    const Reach r = reach_of(a, b, len, i0, i1);
+    int doc_lo = INT_MAX, doc_hi = -1;
+    if (ranges)
+      for (int t = max(r.first, 0) / kDocBlock; t <= min(r.last, a.sk - 1) / kDocBlock && r.first <= r.last && r.last >= 0; ++t) {
+        const int2 x = __ldg(ranges + t);
+        doc_lo = min(doc_lo, x.x & 0x7fffffff);
+        doc_hi = max(doc_hi, x.y);
+      }
+    const int end = (r.keys + kKeys - 1) / kKeys;
+    for (int j = threadIdx.x; j < n_kv; j += kThreads) {
+      bool need = j < end;
+      if (need && ranges) {
+        const int2 x = __ldg(ranges + j);
+        need = (x.x & 0x7fffffff) <= doc_hi && x.y >= doc_lo;
+      }
+      s_need[g * n_kv + j] = need;
+    }
+  }
+  if (threadIdx.x == 0) {
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&q_full[g], 1);
+      mbar_init(&s_full[g], 1); mbar_init(&s_empty[g], 4);
+      mbar_init(&p_full[g], 4); mbar_init(&pv_full[g], 1);
+    }
+    for (int s = 0; s < C::Stages; ++s) {
+      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 2);       // a slot is free once both issuers are done with it
+      mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 2);
+    }
+    mbar_init(v_clean, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  auto next = [&](int j) { while (j < n_kv && !s_need[j] && !s_need[n_kv + j]) ++j; return j; };
+  // the tile that holds both keys of the sequence and rows behind it (rows behind the buffer arrive as zeros anyway)
+  const int ragged = len < a.sk && (len % kKeys) != 0 ? len / kKeys : -1;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLightRegs));
+    if (warp == 0) {
+      if (lane == 0) {
+        for (int g = 0; g < (has_b ? 2 : 1); ++g) {
+          mbar_expect_tx(&q_full[g], C::TileBytes);
+          for (int x = 0; x < C::Boxes; ++x)
+            tma_load_4d(&tmQ, sQ + g * C::TileBytes + x * C::BoxBytes, &q_full[g], x * 64, (2 * pair + g) * kRows, h, b);
+        }
+        int u = 0;
+        for (int j = next(0); j < n_kv; j = next(j + 1), ++u) {
+          const int s = u % C::Stages;
+          if (!mbar_wait(&k_empty[s], ((uint32_t)(u / C::Stages) & 1u) ^ 1u, abort_flag)) break;
+          mbar_expect_tx(&k_full[s], C::TileBytes);
+          for (int x = 0; x < C::Boxes; ++x) tma_load_4d(&tmK, sK + s * C::TileBytes + x * C::BoxBytes, &k_full[s], x * 64, j * kKeys, hk, b);
+        }
+        // the query tiles have landed before this warp may leave
+        for (int g = 0; g < (has_b ? 2 : 1); ++g) mbar_wait(&q_full[g], 0, abort_flag);
+      } else if (lane == 1) {
+        int u = 0;
+        for (int j = next(0); j < n_kv; j = next(j + 1), ++u) {
+          const int s = u % C::Stages;
+          if (!mbar_wait(&v_empty[s], ((uint32_t)(u / C::Stages) & 1u) ^ 1u, abort_flag)) break;
+          mbar_expect_tx(&v_full[s], C::TileBytes);
+          for (int x = 0; x < C::Boxes; ++x) tma_load_4d(&tmV, sV + s * C::TileBytes + x * C::BoxBytes, &v_full[s], x * 64, j * kKeys, hk, b);
+        }
+      }
+    } else if (warp <= 2) {
+      const int g = warp - 1;
+      const unsigned char* need = s_need + g * n_kv;
+      const uint32_t q_addr = smem_u32(sQ + g * C::TileBytes);
+      const uint32_t d_s = tmem_base + (uint32_t)(C::ColS + g * kKeys);
+      const uint32_t d_o = tmem_base + (uint32_t)(C::ColO + g * D);
+      const uint32_t d_p = tmem_base + (uint32_t)(C::ColP + g * C::StepP);
+      const uint32_t idesc_qk = pp.idesc_qk, idesc_pv = pp.idesc_pv;
+      int n_qk = 0, n_pv = 0;
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
+      auto issue_qk = [&](int slot) -> bool {
+        const int n = n_qk++;
+        if (n == 0 && !wait_all(&q_full[g], 0)) return false;
+        if (n > 0 && !wait_all(C::Alias ? &pv_full[g] : &s_empty[g], (uint32_t)(n - 1) & 1u)) return false;
+        tc_fence_after();
+        const uint32_t k_addr = smem_u32(sK + slot * C::TileBytes);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t da = make_kmajor_sw128_desc(q_addr + (uint32_t)((k >> 2) * C::BoxBytes)) + (uint64_t)((k & 3) * 2);
+            const uint64_t db = make_kmajor_sw128_desc(k_addr + (uint32_t)((k >> 2) * C::BoxBytes)) + (uint64_t)((k & 3) * 2);
+            umma<false>(d_s, da, db, idesc_qk, k ? 1u : 0u);
+          }
+          umma_commit(&s_full[g]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_pv = [&](int slot, bool dirty) -> bool {
+        const int n = n_pv++;
+        if (dirty && !wait_all(v_clean, 0)) return false;
+        if (!wait_all(&p_full[g], (uint32_t)n & 1u)) return false;
+        tc_fence_after();
+        const uint32_t v_addr = smem_u32(sV + slot * C::TileBytes);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            // rows of V are the K index: 16 of them are 2048 bytes; the second 64 values of a row lie a box further on
+            uint64_t db = make_mnmajor_sw128_desc(v_addr + (uint32_t)(k * 2048));
+            if (C::Boxes == 2) db = (db & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(C::BoxBytes >> 4) << 16);
+            umma_ts_f16(d_o, d_p + (uint32_t)(k * 8), db, idesc_pv, n > 0 || k > 0 ? 1u : 0u);
+          }
+          umma_commit(&pv_full[g]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto release = [&](uint64_t* bar, bool used) {
+        if (elect_one()) { if (used) umma_commit(bar); else mbar_arrive(bar); }
+        __syncwarp();
+      };
+      // A tile this query tile skips is released once it has landed, so that the arrival counts for that tile.
+      // P of its own: the next scores are issued ahead of P V.  P in the place of the scores: behind it.
+      bool ok = true;
+      int jc = next(0), u = 0;
+      auto scores = [&](int j, int n) {
+        const int slot = n % C::Stages;
+        ok = wait_all(&k_full[slot], (uint32_t)(n / C::Stages) & 1u);
+        const bool used = need[j] != 0;
+        if (ok && used) ok = issue_qk(slot);
+        if (ok) release(&k_empty[slot], used);
+      };
+      if (jc < n_kv) scores(jc, 0);
+      while (jc < n_kv && ok) {
+        const int jn = next(jc + 1);
+        if (!C::Alias && jn < n_kv) scores(jn, u + 1);
+        const int slot = u % C::Stages;
+        if (ok) ok = wait_all(&v_full[slot], (uint32_t)(u / C::Stages) & 1u);
+        const bool used = need[jc] != 0;
+        if (ok && used) ok = issue_pv(slot, jc == ragged);
+        if (ok) release(&v_empty[slot], used);
+        if (C::Alias && ok && jn < n_kv) scores(jn, u + 1);
+        jc = jn;
+        ++u;
+      }
+    } else if (ragged >= 0) {
+      // warp 3: the value rows behind the sequence in its last tile
+      int u = 0, j = next(0);
+      for (; j < n_kv && j != ragged; j = next(j + 1)) ++u;
+      if (j == ragged) {
+        const int slot = u % C::Stages;
+        if (mbar_wait(&v_full[slot], (uint32_t)(u / C::Stages) & 1u, abort_flag)) {
+          const int r0 = len - ragged * kKeys;
+          for (int i = lane; i < (kKeys - r0) * 8 * C::Boxes; i += 32) {      // a row is 128 bytes of each box, wherever its pieces lie
+            const int x = i / ((kKeys - r0) * 8), c = i - x * ((kKeys - r0) * 8);
+            *reinterpret_cast<uint4*>(sV + slot * C::TileBytes + x * C::BoxBytes + r0 * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_clean);
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int g = (warp - 4) >> 2, quarter = warp & 3;
+    const int r_in_tile = quarter * 32 + lane;
+    const int row = (2 * pair + g) * kRows + r_in_tile;
+    const bool active = g == 0 || has_b, row_ok = active && row < a.sq;
+    if (active) {
+      const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
+      const uint32_t t_s = tmem_base + (uint32_t)(C::ColS + g * kKeys) + lane_sel;
+      const uint32_t t_o = tmem_base + (uint32_t)(C::ColO + g * D) + lane_sel;
+      const uint32_t t_p = tmem_base + (uint32_t)(C::ColP + g * C::StepP) + lane_sel;
+      const unsigned char* need = s_need + g * n_kv;
+      const Reach me = reach_of(a, b, len, row, row_ok ? row : row - 1);
+      int hi = me.keys, doc = -1;
+      if (docs) {
+        doc = me.keys > 0 && me.first >= 0 && me.first < a.sk ? __ldg(docs + me.first) : -1;
+        if (doc < 0) hi = 0;
+      }
+      const int pos = me.first;
+      const float slope = BIAS && a.slopes ? a.slopes[h] * kLog2e : 0.f;
+      const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_cap = CAP ? a.scale / a.cap : 0.f;
+      constexpr bool FOLD = !CAP && !BIAS;        // the scale is applied in the exponent (it is positive then)
+      float m_ref = -CUDART_INF_F, l = 0.f;
+      bool ok = true;
+      int t = 0;
+      for (int j = 0; j < n_kv && ok; ++j) {
+        if (!need[j]) continue;
+        const int k0 = j * kKeys;
+        bool whole = hi >= k0 + kKeys;
+        if (docs) {
+          const int2 x = __ldg(ranges + j);
+          whole = whole && x.x == doc && x.y == doc;      // a block with keys of no document has its sign bit set
+        }
+        const bool hide = !__all_sync(0xffffffffu, whole);
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g], (uint32_t)t & 1u, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        float x[kKeys];
+        uint32_t* xu = reinterpret_cast<uint32_t*>(x);
+        tmem_ld32_issue(t_s, xu);
+        tmem_ld32_issue(t_s + 32, xu + 32);
+        tmem_ld32_issue(t_s + 64, xu + 64);
+        tmem_ld32_issue(t_s + 96, xu + 96);
+        tmem_ld_wait();
+        float base = 0.f;                                  // added to every score of the row
+        if (CAP) {
+          float z0 = 0.f, z1 = 0.f;
+#pragma unroll
+          for (int i = 0; i < kKeys; i += 2) {
+            mul2(x[i], x[i + 1], x[i], x[i + 1], to_cap, to_cap);
+            if (i & 2) z1 = fmax3(z1, fabsf(x[i]), fabsf(x[i + 1]));
+            else z0 = fmax3(z0, fabsf(x[i]), fabsf(x[i + 1]));
+          }
+          if (__all_sync(0xffffffffu, fmaxf(z0, z1) <= 1.0f)) {
+            // tanh(x) = x P(x^2) on [-1, 1], fitted to a largest relative error of 6.2e-7
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 2) {
+              float z, y, q, r;
+              mul2(z, y, x[i], x[i + 1], x[i], x[i + 1]);
+              fma2(q, r, z, y, -0.003067060373723507f, -0.003067060373723507f, 0.016743116080760956f, 0.016743116080760956f);
+              fma2(q, r, z, y, q, r, -0.051605675369501114f, -0.051605675369501114f);
+              fma2(q, r, z, y, q, r, 0.13281433284282684f, 0.13281433284282684f);
+              fma2(q, r, z, y, q, r, -0.3332904279232025f, -0.3332904279232025f);
+              fma2(q, r, z, y, q, r, 0.9999994039535522f, 0.9999994039535522f);
+              mul2(x[i], x[i + 1], x[i], x[i + 1], to_log2, to_log2);
+              mul2(x[i], x[i + 1], x[i], x[i + 1], q, r);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i)
+              x[i] = to_log2 * (1.0f - __fdividef(2.0f, 1.0f + ex2_approx(x[i] * (2.0f * kLog2e))));
+          }
+        } else if (BIAS) {
+#pragma unroll
+          for (int i = 0; i < kKeys; i += 2) mul2(x[i], x[i + 1], x[i], x[i + 1], to_log2, to_log2);
+        }
+        if (BIAS) {
+          if (__all_sync(0xffffffffu, k0 + kKeys - 1 <= pos)) {        // every key behind the row: the distance is linear
+            base = slope * (float)(k0 - pos);
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) x[i] = fmaf(slope, (float)i, x[i]);
+          } else {
+            const float gap = (float)(pos - k0);
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) x[i] = fmaf(-slope, fabsf(gap - (float)i), x[i]);
+          }
+        }
+        uint32_t dead = 0u;                                 // 32-key pieces that no row of this warp sees
+        if (hide) {
+          tmem_st32_issue(t_s, xu);
+          tmem_st32_issue(t_s + 32, xu + 32);
+          tmem_st32_issue(t_s + 64, xu + 64);
+          tmem_st32_issue(t_s + 96, xu + 96);
+          tmem_st_wait();
+          const int n = min(max(hi - k0, 0), kKeys);
+          uint32_t w[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) w[c] = n >= 32 * c + 32 ? 0xffffffffu : n <= 32 * c ? 0u : (1u << (n - 32 * c)) - 1u;
+          uint4 seen = make_uint4(w[0], w[1], w[2], w[3]);
+          if (docs) {
+            const uint4 mine = document_bits(docs + k0, min(a.sk - k0, kKeys), doc);
+            seen = make_uint4(seen.x & mine.x, seen.y & mine.y, seen.z & mine.z, seen.w & mine.w);
+          }
+          dead = __reduce_and_sync(0xffffffffu, hide_scores(t_s, seen));
+          tmem_ld32_issue(t_s, xu);
+          tmem_ld32_issue(t_s + 32, xu + 32);
+          tmem_ld32_issue(t_s + 64, xu + 64);
+          tmem_ld32_issue(t_s + 96, xu + 96);
+          tmem_ld_wait();
+        }
+        if (!C::Alias) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[g]);
+        }
+        float mt;
+        {
+          float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int i = 4; i < kKeys; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], x[i], x[i + 1]);
+          mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          if (FOLD) mt *= to_log2;
+          else mt += base;
+        }
+        // O is rescaled by whole warps once the P V before it has completed (with P in the place of the scores these
+        // scores are younger than that product)
+        bool pv_done = t == 0 || C::Alias;
+        const bool raise = m_ref != -CUDART_INF_F && mt - m_ref > kLazyLog2;
+        if (__any_sync(0xffffffffu, raise)) {
+          if (!pv_done) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&pv_full[g], (uint32_t)(t - 1) & 1u, abort_flag));
+            if (!ok) break;
+            pv_done = true;
+            tc_fence_after();
+          }
+          const float alpha = raise ? ex2_approx(m_ref - mt) : 1.0f;
+          rescale_row<D>(t_o, alpha);
+          if (raise) { l *= alpha; m_ref = mt; }
+        }
+        if (m_ref == -CUDART_INF_F) m_ref = mt;
+        const float off = (m_ref == -CUDART_INF_F ? 0.f : -m_ref) + base;
+        {
+          float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < kKeys / 32; ++c) {
+            if ((dead >> c) & 1u) {
+#pragma unroll
+              for (int i = c * 32; i < c * 32 + 32; ++i) x[i] = 0.f;
+            } else {
+#pragma unroll
+              for (int i = c * 32; i < c * 32 + 32; i += 2) {
+                if (FOLD) fma2(x[i], x[i + 1], x[i], x[i + 1], to_log2, to_log2, off, off);
+                else add2(x[i], x[i + 1], x[i], x[i + 1], off, off);
+                x[i] = ex2_approx(x[i]);
+                x[i + 1] = ex2_approx(x[i + 1]);
+                add2(ps[i & 2], ps[(i & 2) + 1], ps[i & 2], ps[(i & 2) + 1], x[i], x[i + 1]);
+              }
+            }
+          }
+          l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        }
+        if (!pv_done) {             // P of the previous key tile has been consumed
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_full[g], (uint32_t)(t - 1) & 1u, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = pack16<BF16>(x[half * 64 + 2 * i], x[half * 64 + 2 * i + 1]);
+          tmem_st32_issue(t_p + (uint32_t)(half * 32), w);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
+        ++t;
+      }
+      if (ok && t > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pv_full[g], (uint32_t)(t - 1) & 1u, abort_flag));
+      if (ok) {
+        tc_fence_after();
+        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);      // a row without keys is zero; NaN stays NaN
+        uint16_t* out = reinterpret_cast<uint16_t*>(const_cast<void*>(a.out.ptr)) + b * a.out.sb + (long long)h * a.out.sh + (long long)(row_ok ? row : 0) * a.out.sr;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          if (t > 0) tmem_ld32(t_o + (uint32_t)(c * 32), r);
+          if (row_ok) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              if (c * 32 + i >= a.d) continue;
+              float o[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[e] = t > 0 && l != 0.f ? __uint_as_float(r[i + e]) * inv : 0.f;
+              *reinterpret_cast<uint4*>(out + c * 32 + i) =
+                  make_uint4(pack16<BF16>(o[0], o[1]), pack16<BF16>(o[2], o[3]), pack16<BF16>(o[4], o[5]), pack16<BF16>(o[6], o[7]));
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) { *a.status.host = BG_ERR_DEVICE_TIMEOUT; *a.status.device = BG_ERR_DEVICE_TIMEOUT; }
+    const long long t0 = clock64();
+    while (clock64() - t0 < 200000) {}
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(p);
+    cudaGetLastError();
+    return (EncodeTiledFn) nullptr;
+  }();
+  return fn;
+}
+
+// Boxes of 128 rows x 64 values with the 128-byte swizzle; values behind d and rows behind the last arrive as zeros.
+bool make_map(CUtensorMap* map, const HeadPtr& v, int dtype, int b, int rows, int heads, int d) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)b};
+  // an axis of extent one has no stride: any legal value will do
+  const cuuint64_t any = ((cuuint64_t)d * 2 + 15) / 16 * 16;
+  cuuint64_t strides[3] = {rows > 1 ? (cuuint64_t)v.sr * 2 : any, heads > 1 ? (cuuint64_t)v.sh * 2 : any, b > 1 ? (cuuint64_t)v.sb * 2 : any};
+  cuuint32_t box[4] = {64, 128, 1, 1}, step[4] = {1, 1, 1, 1};
+  return fn(map, dtype == BG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(v.ptr), dims, strides,
+            box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What TMA asks of a view: 16-byte steps below 2^40 bytes, no axis that stands still.
+bool view_fits(const HeadPtr& v, int b, int rows, int heads) {
+  if (reinterpret_cast<uintptr_t>(v.ptr) & 15) return false;
+  const int64_t st[3] = {v.sr, v.sh, v.sb};
+  const int ext[3] = {rows, heads, b};
+  for (int i = 0; i < 3; ++i)
+    if (ext[i] > 1 && (st[i] <= 0 || st[i] % 8 || st[i] >= ((int64_t)1 << 38))) return false;
+  return true;
+}
+
+template <int D>
+size_t smem_bytes(int sk) { return (size_t)Cfg<D>::Smem + 1024 + 256 + 2 * (size_t)((sk + kKeys - 1) / kKeys); }
+
+template <bool BF16, int D, bool CAP, bool BIAS>
+cudaError_t launch_kernel(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
+  auto kern = prompt_attention_kernel<BF16, D, CAP, BIAS>;
+  cudaFuncAttributes fa;
+  cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+  if (e != cudaSuccess) return e;
+  if (fa.numRegs < kLaunchRegs) return cudaErrorLaunchOutOfResources;
+  const size_t smem = smem_bytes<D>(p.a.sk);
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const int pairs = ((p.a.sq + kRows - 1) / kRows + 1) / 2;
+  kern<<<(unsigned)((long long)pairs * p.a.b * p.a.hq), kThreads, smem, s>>>(q, k, v, p);
+  return cudaGetLastError();
+}
+
+template <bool BF16, int D>
+cudaError_t launch_rules(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
+  // a scale that is not positive cannot be taken out of the row maximum: such scores are scaled like biased ones
+  const bool bias = p.a.slopes || !(p.a.scale > 0.f), cap = p.a.cap > 0.f;
+  if (cap) return bias ? launch_kernel<BF16, D, true, true>(p, q, k, v, s) : launch_kernel<BF16, D, true, false>(p, q, k, v, s);
+  return bias ? launch_kernel<BF16, D, false, true>(p, q, k, v, s) : launch_kernel<BF16, D, false, false>(p, q, k, v, s);
+}
+
+}  // namespace
+
+bool prompt_attention_usable(const DecoderAttention& p, int dtype) {
+  if ((dtype != BG_BF16 && dtype != BG_F16) || p.d > 128 || p.d % 8 || p.sk == 0 || !encode_fn()) return false;
+  // Below 64 rows a head most of a 128-row tile would stand empty, and the key-split kernel reads each key once for the
+  // whole group.
+  if (p.sq < 64) return false;
+  if (smem_bytes<128>(p.sk) > 227 * 1024) return false;
+  if ((long long)((p.sq + 255) / 256) * p.b * p.hq > 0x7fffffffll) return false;
+  return view_fits(p.q, p.b, p.sq, p.hq) && view_fits(p.k, p.b, p.sk, p.hkv) && view_fits(p.v, p.b, p.sk, p.hkv) && view_fits(p.out, p.b, p.sq, p.hq);
+}
+
+cudaError_t launch_prompt_attention(const DecoderAttention& p, int dtype, cudaStream_t s) {
+  CUtensorMap q, k, v;
+  if (!make_map(&q, p.q, dtype, p.b, p.sq, p.hq, p.d) || !make_map(&k, p.k, dtype, p.b, p.sk, p.hkv, p.d) || !make_map(&v, p.v, dtype, p.b, p.sk, p.hkv, p.d))
+    return cudaErrorInvalidValue;
+  const bool bf = dtype == BG_BF16, wide = p.d > 64;
+  const uint32_t fmt = bf ? 1u : 0u;
+  PromptParams pp;
+  pp.a = p;
+  pp.idesc_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+  pp.idesc_pv = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)((wide ? 128 : 64) >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);   // V is MN-major
+  if (wide) return bf ? launch_rules<true, 128>(pp, q, k, v, s) : launch_rules<false, 128>(pp, q, k, v, s);
+  return bf ? launch_rules<true, 64>(pp, q, k, v, s) : launch_rules<false, 64>(pp, q, k, v, s);
+}
+
+}  // namespace bg

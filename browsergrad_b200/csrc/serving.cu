@@ -353,6 +353,12 @@ int decoder_attention(const Call& c, const bg_head_view* q, const bg_head_view* 
       p.doc_ranges = reinterpret_cast<const int2*>(ranges.p);
       if (int rc = launch(c, "doc_ranges", 1, [&] { return launch_doc_ranges(documents, p.b, p.sk, reinterpret_cast<int2*>(ranges.p), c.ctx->stream); })) return rc;
     }
+    if (prompt_attention_usable(p, dtype)) {
+      if (int rc = launch(c, std::string("prompt_attention[") + dtype_name(dtype) + "]", 1, [&] { return launch_prompt_attention(p, dtype, c.ctx->stream); })) return rc;
+      c.ctx->status_pending = true;
+      *out = keep(&r, dtype, b, sq, hq, d);
+      return BG_OK;
+    }
     const CacheAttnPlan plan = cache_attention_plan(p, dtype, c.ctx->sm_count);
     if (plan.partial_bytes)
       if (int rc = partials.get(plan.partial_bytes)) return rc;

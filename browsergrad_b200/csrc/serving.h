@@ -52,7 +52,8 @@ struct DecoderAttention {
   const int* lengths;         // [b] or null (then sk)
   const int* starts;          // [b] or null (then lengths[b] - sq)
   int causal;
-  const int2* doc_ranges;     // [b, ceil(sk / 128)] smallest and largest id of each 128 keys; set with documents
+  const int2* doc_ranges;     // [b, ceil(sk / 128)] smallest and largest id of each 128 keys, the smallest with its sign bit
+                              // set when some of them belong to no document; set with documents
   StatusWords status;
 };
 constexpr int kDocBlock = 128;
@@ -67,6 +68,10 @@ struct CacheAttnPlan {
 CacheAttnPlan cache_attention_plan(const DecoderAttention& p, int dtype, int sm_count);
 cudaError_t launch_cache_attention(const DecoderAttention& p, int dtype, const CacheAttnPlan& plan, float* partials, int* counters,
                                    cudaStream_t s);
+
+// Prompts of 16-bit operands (prompt_attn.cu).
+bool prompt_attention_usable(const DecoderAttention& p, int dtype);
+cudaError_t launch_prompt_attention(const DecoderAttention& p, int dtype, cudaStream_t s);
 
 // ---- sample.cu ---------------------------------------------------------------------------------------------------
 struct SampleProblem {
