@@ -6,13 +6,15 @@
 //
 // A row is read once: a cluster of up to eight CTAs shares it and each keeps its slice in shared memory as ordered 32-bit
 // keys (rows too long for that are read again from L2 instead).  No sort: the rank and the sum are thresholds on the
-// value, found by histograms over ever narrower ranges of keys -- 2048 buckets, the first round linear in the value so
-// that the bulk of a row does not meet in a few buckets -- and what is left at the threshold itself are equal values,
-// taken in index order.  Each round ends in one cluster barrier.
+// value.  A histogram of 2048 buckets, linear in the value so that the bulk of a row does not meet in a few of them, gives
+// the bucket a threshold lies in, whose keys are collected and sorted (where top-k leaves few keys, all the kept ones are
+// collected, and the rest of the work is comparing all pairs).  A bucket with too many keys for that is narrowed by further
+// histograms over its range of keys until equal values are left, which are taken in index order.
 // Weights are whole numbers, round(w 2^46) (fewer bits for a vocabulary whose sum would pass 2^62): sums are then exact,
-// the same in any order, so atomics cannot change the result.  A weight is off by at most 2^-47 of the largest and a
-// running sum by some 2^-47 sqrt(V), while u has 24 bits; 32-bit weights would move one choice in a thousand.  Exponentials
-// are 64-bit, and the part of a row that is below 2^-47 is skipped ahead of them.
+// the same in any order, so atomics cannot change the result.  A weight is off by at most 2^-46 of the largest and a
+// running sum by some 2^-46 sqrt(V), while u has 24 bits; 32-bit weights would move one choice in a thousand.  The
+// exponential is 64-bit: 2^y = 2^(i / 256) (from a table) e^t, |t| <= ln 2 / 512, the last factor by its series to t^4
+// (4 * 10^-17 dropped), a dozen operations against some forty of the general function.
 #include "serving.h"
 
 #include <cooperative_groups.h>
@@ -29,6 +31,8 @@ typedef unsigned long long u64;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBuckets = 2048, kCoarse = 64;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxListed = 1024;     // keys of one bucket that are sorted
+constexpr int kMaxPairs = 256;       // keys that are ranked by comparing all pairs
 
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
@@ -44,19 +48,36 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k
 
 constexpr uint32_t kLowestKey = 0x00800000u;           // of the lowest finite value
 
+// A bucket's sum in two words: 64-bit atomics on shared memory are a loop (1.1 a clock and SM measured, 32-bit ones 4.8), and
+// a weight below 2^-14 touches the upper word only with its carry.
 struct Shared {
-  u64 hist[2][kBuckets];
-  u64 coarse[2][kCoarse];
-  u64 seg_sum[kWarps];
+  uint32_t low[kBuckets], high[kBuckets];
+  uint32_t counts[kBuckets];           // keys of each bucket
+  u64 coarse[kCoarse];
+  u64 listed[kMaxListed];              // this CTA's keys of a bucket: key << 32 | ~index, so that larger means ranked earlier
+  u64 pair_weight[kMaxPairs];
+  double table[256];                   // 2^(i / 256)
+  u64 seg_sum[kWarps], warp_sum[kWarps];
   uint32_t seg_ties[kWarps];
-  uint32_t top, low, first;            // this CTA's part of a cluster-wide maximum, minimum, first index
+  uint32_t top, bottom, first;         // this CTA's part of a cluster-wide maximum, minimum, first index
   uint32_t warp_a[kWarps], warp_b[kWarps];
-  // what one warp found for all
-  uint32_t bucket, all_top, all_low, all_first;
+  uint32_t n_listed;
+  // what one warp or thread found for all
+  uint32_t all_top, all_bottom;
+  uint32_t bucket, in_bucket;
   u64 above, total, rest;
   int seg;
   uint32_t seg_tie_base;
+  uint32_t cut_key, cut_ties;
+  // the cluster's list, in the place of the sums: they have been read by then (collect())
+  __device__ u64* all_listed() { return reinterpret_cast<u64*>(low); }
+  __device__ void add(uint32_t b, u64 f) {
+    const uint32_t v = (uint32_t)f, old = atomicAdd(&low[b], v);
+    const uint32_t h = (uint32_t)(f >> 32) + (old + v < old ? 1u : 0u);
+    if (h) atomicAdd(&high[b], h);
+  }
 };
+static_assert(kMaxListed * 8 <= 2 * kBuckets * 4, "the list fits where the sums were");
 
 // Kept: keys above `key`, and the first `ties` of those equal to it.
 struct Cut {
@@ -66,22 +87,33 @@ struct Cut {
 struct Row {
   uint32_t top;            // largest key
   float top_value;
-  double top_wide, inv_t;
-  float inv_t32;
+  double top_wide, step;   // 256 / (T ln 2)
+  double one, floor;       // weight of the largest, 2^bits; and the smallest weight min_p keeps
   int bits;                // fraction bits of a weight
-  float min_p;
-  __device__ double weight(uint32_t k) const {
-    if (k == top) return 1.0;
-    if (k == 0u || isinf(top_value)) return 0.0;
-    const float x = value_of(k);
-    if ((x - top_value) * inv_t32 < -34.0f) return 0.0;     // rounds to zero
-    return exp(((double)x - top_wide) * inv_t);
+  bool finite;             // the largest is not +inf
+  const double* table;
+  // the weight times 2^bits, before its rounding (k > 0)
+  __device__ __forceinline__ double scaled(uint32_t k) const {
+    const double magic = 6755399441055744.0;                // 1.5 * 2^52: its sum with a small number rounds it to a whole one
+    double y = ((double)value_of(k) - top_wide) * step;
+    y = y > -12800.0 ? y : -12800.0;                        // 2^-50 and less, which 2^46 times rounds to zero; NaN too
+    const double s = y + magic;
+    const int n = __double2loint(s);
+    const double r = y - (s - magic);                       // y = n + r, |r| <= 1/2
+    const double u = 0.0027076061740622863;                 // ln 2 / 256
+    double q = fma(r, u * u * u * u / 24.0, u * u * u / 6.0);
+    q = fma(r, q, u * u / 2.0);
+    q = fma(r, q, u);
+    const double t = table[n & 255];
+    const double w = fma(t, r * q, t);
+    const double e = __hiloint2double(__double2hiint(w) + (((n >> 8) + bits) << 20), __double2loint(w));
+    return finite ? e : (k == top ? one : 0.0);
   }
-  __device__ u64 fixed(double w) const { return (u64)(w * (double)(1ull << bits) + 0.5); }
-  __device__ u64 fixed_of(uint32_t k) const { return fixed(weight(k)); }
+  __device__ u64 fixed(double w) const { return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull; }     // to nearest, w < 2^51
+  __device__ u64 fixed_of(uint32_t k) const { return fixed(scaled(k)); }
   __device__ u64 drawn(uint32_t k) const {                  // weight in the final draw: min_p applied
-    const double w = weight(k);
-    return k == top || w >= (double)min_p ? fixed(w) : 0ull;
+    const double w = scaled(k);
+    return k == top || w >= floor ? fixed(w) : 0ull;
   }
 };
 
@@ -121,6 +153,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
   // ---- read the slice; largest and smallest key ----
   uint32_t top = 0u, low = 0xffffffffu;
+  for (int i = tid; i < kBuckets; i += kThreads) { sh.low[i] = 0u; sh.high[i] = 0u; sh.counts[i] = 0u; }
+  if (tid < 256) sh.table[tid] = exp2((double)tid / 256.0);
+  if (tid == 0) sh.n_listed = 0u;
+#pragma unroll 4
   for (int j = tid * VEC; j < slice; j += kThreads * VEC) {
     const int64_t e = begin + j;
     uint32_t k[VEC];
@@ -149,18 +185,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (warp == 0) {
     top = __reduce_max_sync(0xffffffffu, lane < kWarps ? sh.warp_a[lane] : 0u);
     low = __reduce_min_sync(0xffffffffu, lane < kWarps ? sh.warp_b[lane] : 0xffffffffu);
-    if (lane == 0) { sh.top = top; sh.low = low; }
+    if (lane == 0) { sh.top = top; sh.bottom = low; }
   }
   cluster.sync();
   if (warp == 0) {
     const Shared* r = cluster.map_shared_rank(&sh, lane < nc ? lane : 0);
     top = __reduce_max_sync(0xffffffffu, r->top);
-    low = __reduce_min_sync(0xffffffffu, r->low);
-    if (lane == 0) { sh.all_top = top; sh.all_low = low; }
+    low = __reduce_min_sync(0xffffffffu, r->bottom);
+    if (lane == 0) { sh.all_top = top; sh.all_bottom = low; }
   }
   __syncthreads();
   top = sh.all_top;
-  low = sh.all_low;
+  low = sh.all_bottom;
 
   const float t = p.temperatures ? p.temperatures[row] : p.temperature;
   if (top == 0u || !(t > 0.0f)) {
@@ -192,36 +228,53 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   w.top = top;
   w.top_value = value_of(top);
   w.top_wide = (double)w.top_value;
-  w.inv_t = 1.0 / (double)t;
-  w.inv_t32 = (float)w.inv_t;
+  w.finite = w.top_value < CUDART_INF_F;
+  w.step = 369.3299304675746 / (double)t;                 // 256 / ln 2
   w.bits = min(46, 62 - (64 - __clzll((long long)p.vocab)));
-  w.min_p = p.min_ps ? p.min_ps[row] : p.min_p;
-  w.min_p = w.min_p > 0.0f ? fminf(w.min_p, 1.0f) : 0.0f;
+  w.one = (double)(1ull << w.bits);
+  w.table = sh.table;
+  const float min_p = p.min_ps ? p.min_ps[row] : p.min_p;
+  w.floor = min_p > 0.0f ? w.one * (double)fminf(min_p, 1.0f) : 0.0;
+  float u = p.uniforms[row];
+  u = u > 0.0f ? u : 0.0f;
+  // what the running sum has to exceed
+  auto draw_target = [&](u64 total) -> u64 {
+    const u64 at = u < 1.0f ? (u64)((double)u * (double)total) : total;
+    return at < total ? at : total - 1;
+  };
 
   int round = 0;
-  // One round: `add(key, hist)` for this CTA's keys and `once(hist)` for the cluster, then the bucket in which the running
-  // sum (bucket 0 first) reaches the target.  target_of(total) gives the target from the round's total.
-  auto search = [&](auto&& add, auto&& once, auto&& target_of) {
-    const int par = round & 1;
+  // One round: `add(key)` for this CTA's keys and `once()` for the cluster, then the bucket
+  // in which the running sum (bucket 0 first) reaches the target.  target_of(total) gives the target from the round's
+  // total.  Counts are the sums of a round that counts.
+  auto search = [&](bool counting, auto&& add, auto&& once, auto&& target_of) {
+    if (round > 0) {
+      cluster.sync();                        // the other CTAs have read the last round's
+      for (int i = tid; i < kBuckets; i += kThreads) { sh.low[i] = 0u; sh.high[i] = 0u; sh.counts[i] = 0u; }
+      __syncthreads();
+    }
     ++round;
-    u64* hist = sh.hist[par];
-    for (int i = tid; i < kBuckets; i += kThreads) hist[i] = 0ull;
+    if (rank == 0 && tid == 0) once();
+#pragma unroll 4
+    for (int j = tid; j < slice; j += kThreads) add(key_at(j));
     __syncthreads();
-    if (rank == 0 && tid == 0) once(hist);
-    for (int j = tid; j < slice; j += kThreads) add(key_at(j), hist);
-    __syncthreads();
-    for (int c = warp; c < kCoarse; c += kWarps) {
-      const u64 s = warp_sum(hist[c * 32 + lane]);
-      if (lane == 0) sh.coarse[par][c] = s;
+#pragma unroll
+    for (int i = 0; i < kCoarse / kWarps; ++i) {
+      const int c = warp + i * kWarps;
+      const int i32 = c * 32 + lane;
+      const u64 s = counting ? (u64)__reduce_add_sync(0xffffffffu, sh.counts[i32]) : warp_sum((u64)sh.high[i32] << 32 | sh.low[i32]);
+      if (lane == 0) sh.coarse[c] = s;
     }
     cluster.sync();
     if (warp == 0) {
       u64 a = 0, b = 0;
-      for (int r = 0; r < nc; ++r) {
-        const u64* q = cluster.map_shared_rank(&sh, r)->coarse[par];
-        a += q[2 * lane];
-        b += q[2 * lane + 1];
-      }
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < nc) {
+          const ulonglong2 q = reinterpret_cast<const ulonglong2*>(cluster.map_shared_rank(&sh, r)->coarse)[lane];
+          a += q.x;
+          b += q.y;
+        }
       const u64 incl = warp_scan(a + b, lane);
       const u64 total = __shfl_sync(0xffffffffu, incl, 31);
       u64 target = target_of(total);
@@ -233,7 +286,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       int c = 2 * at;
       if (above + a_at < target) { above += a_at; ++c; }
       u64 f = 0;
-      for (int r = 0; r < nc; ++r) f += cluster.map_shared_rank(&sh, r)->hist[par][c * 32 + lane];
+      uint32_t n = 0;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < nc) {
+          const Shared* q = cluster.map_shared_rank(&sh, r);
+          if (!counting) f += (u64)q->high[c * 32 + lane] << 32 | q->low[c * 32 + lane];
+          n += q->counts[c * 32 + lane];
+        }
+      if (counting) f = n;
       const u64 fi = warp_scan(f, lane);
       const int fl = __ffs(__ballot_sync(0xffffffffu, above + fi >= target)) - 1;
       if (lane == fl) {
@@ -241,40 +302,95 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         sh.above = above + fi - f;
         sh.total = total;
         sh.rest = target - (above + fi - f);       // how much of the bucket is wanted
+        sh.in_bucket = n;
       }
     }
     __syncthreads();
   };
-  // Narrows [lo, hi] until one key is left: the key at which the sum of `amount(key)` over the kept keys, largest first,
-  // reaches the target; returns what is wanted of that key's own group.
-  auto threshold = [&](float x_low, bool counting, Cut cut, auto&& target_of, uint32_t* key) -> u64 {
-    const float span = w.top_value - x_low;
-    const float sc = span > 0.0f && span < CUDART_INF_F ? (float)kBuckets / span : 0.0f;
-    auto linear = [&](uint32_t k) -> uint32_t {         // never increases with the key
-      const float v = (w.top_value - value_of(k)) * sc;
-      return v >= (float)(kBuckets - 1) ? kBuckets - 1 : (uint32_t)(int)v;      // NaN (infinite top) becomes bucket 0
-    };
-    auto amount = [&](uint32_t k, u64* slot) {
-      if (counting) atomicAdd(reinterpret_cast<unsigned int*>(slot), 1u);       // the low word: counts stay below 2^31
-      else if (const u64 f = w.fixed_of(k)) atomicAdd(slot, f);
-    };
-    auto cut_ties = [&](uint32_t lo, uint32_t hi, auto&& bucket_of, u64* hist) {  // the kept ones of the earlier cut, together
-      if (!counting && cut.ties && cut.key >= lo && cut.key <= hi) {
-        const u64 f = w.fixed_of(cut.key) * cut.ties;
-        if (f) atomicAdd(&hist[bucket_of(cut.key)], f);
+  // Collects the cluster's keys that `wanted` names (at most kMaxListed, the caller knows) into all_listed; returns their
+  // number.  `n_listed` is zero before; the lists may be read until the next cluster barrier.
+  auto collect = [&](auto&& wanted) -> int {
+    for (int j = tid; j < slice; j += kThreads) {
+      const uint32_t k = key_at(j);
+      if (k && wanted(k)) {
+        const uint32_t at = atomicAdd(&sh.n_listed, 1u);
+        if (at < kMaxListed) sh.listed[at] = (u64)k << 32 | (uint32_t)~(uint32_t)(begin + j);
       }
-    };
-    search([&](uint32_t k, u64* hist) { if (k > cut.key) amount(k, &hist[linear(k)]); },
-           [&](u64* hist) { cut_ties(kLowestKey, w.top, linear, hist); }, target_of);
+    }
+    cluster.sync();
+    u64* all = sh.all_listed();
+    uint32_t n = 0;
+    for (int r = 0; r < nc; ++r) {
+      const Shared* q = cluster.map_shared_rank(&sh, r);
+      const uint32_t m = q->n_listed;
+      for (uint32_t i = tid; i < m && n + i < kMaxListed; i += kThreads) all[n + i] = q->listed[i];
+      n += m;
+    }
+    __syncthreads();
+    return (int)min(n, (uint32_t)kMaxListed);
+  };
+  // The value at which the sum of what the kept keys count for (one, or their weights), largest first, reaches a target.
+  auto linear_of = [&](float x_low) -> float {
+    const float span = w.top_value - x_low;
+    return span > 0.0f && span < CUDART_INF_F ? (float)kBuckets / span : 0.0f;
+  };
+  auto linear = [&](uint32_t k, float sc) -> uint32_t {   // never increases with the key
+    const float v = (w.top_value - value_of(k)) * sc;
+    return v >= (float)(kBuckets - 1) ? kBuckets - 1 : (uint32_t)(int)v;      // NaN (infinite top) becomes bucket 0
+  };
+  // From the bucket a first round found: the cut among its keys.  `before` is what lies above the bucket, sh.rest what
+  // is wanted of it.
+  auto resolve = [&](float sc, bool counting, Cut cut) -> Cut {
     const uint32_t b0 = sh.bucket;
     u64 wanted = sh.rest;
+    const uint32_t held = sh.in_bucket;
+    const bool splits_ties = !counting && cut.ties && linear(cut.key, sc) == b0;     // then the earlier cut's own ties are in it
+    if (held <= kMaxListed && !splits_ties) {
+      const int n = collect([&](uint32_t k) { return k > cut.key && linear(k, sc) == b0 && (counting || w.fixed_of(k)); });
+      u64* all = sh.all_listed();
+      const int padded = n <= 1 ? 1 : 1 << (32 - __clz(n - 1));
+      for (int i = n + tid; i < padded; i += kThreads) all[i] = 0ull;
+      // bitonic, largest first
+      for (int size = 2; size <= padded; size *= 2)
+        for (int d = size / 2; d; d /= 2) {
+          __syncthreads();
+          for (int i = tid; i < padded / 2; i += kThreads) {
+            const int x = (i / d) * 2 * d + i % d, y = x + d;
+            const u64 p0 = all[x], p1 = all[y];
+            if ((p0 < p1) == ((x & size) == 0)) { all[x] = p1; all[y] = p0; }
+          }
+        }
+      __syncthreads();
+      // running sums of two neighbours a thread; the one that reaches what is wanted is the cut
+      const int i0 = 2 * tid;
+      const u64 e0 = i0 < n ? all[i0] : 0ull, e1 = i0 + 1 < n ? all[i0 + 1] : 0ull;
+      const u64 f0 = !e0 ? 0ull : counting ? 1ull : w.fixed_of((uint32_t)(e0 >> 32)), f1 = !e1 ? 0ull : counting ? 1ull : w.fixed_of((uint32_t)(e1 >> 32));
+      const u64 in_warp = warp_scan(f0 + f1, lane);
+      if (lane == 31) sh.warp_sum[warp] = in_warp;
+      __syncthreads();
+      u64 before = in_warp - f0 - f1;
+      for (int i = 0; i < warp; ++i) before += sh.warp_sum[i];
+      int at = -1;
+      if (before < wanted && before + f0 >= wanted) at = i0;
+      else if (before + f0 < wanted && before + f0 + f1 >= wanted) at = i0 + 1;
+      if (at >= 0) {                       // exactly one thread
+        const uint32_t key = (uint32_t)(all[at] >> 32);
+        uint32_t same = 1;
+        while ((int)same <= at && (uint32_t)(all[at - (int)same] >> 32) == key) ++same;
+        sh.cut_key = key;
+        sh.cut_ties = same;
+      }
+      cluster.sync();                      // every list has been read, the cut is there
+      if (tid == 0) sh.n_listed = 0u;
+      return Cut{sh.cut_key, sh.cut_ties};
+    }
     // the keys of that bucket: [smallest key in a bucket <= b0, smallest key in a bucket < b0), 32 probes at a time
     auto smallest = [&](uint32_t bucket) {              // smallest key of a number whose bucket is at most `bucket`
-      uint32_t a = kLowestKey, z = w.top;                       // the answer lies in [a, z]
+      uint32_t a = kLowestKey, z = w.top;               // the answer lies in [a, z]
       while (a < z) {
         const uint32_t step = (z - a) / 33u + 1u;
         const uint32_t at = z - a > step * (uint32_t)lane ? a + step * (uint32_t)lane : z;
-        const uint32_t yes = __ballot_sync(0xffffffffu, linear(at) <= bucket);
+        const uint32_t yes = __ballot_sync(0xffffffffu, linear(at, sc) <= bucket);
         const int l = __ffs(yes) - 1;                   // probes grow with the lane; the first that qualifies
         if (l < 0) { a = min(z, a + 31u * step) + 1u; if (a > z) a = z; }
         else {
@@ -290,36 +406,100 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       const int shift = max(0, 21 - __clz(hi - lo));     // 2048 buckets over the range
       auto bucket_of = [&](uint32_t k) { return (hi - k) >> shift; };
       const u64 want = wanted;
-      search([&](uint32_t k, u64* hist) { if (k >= lo && k <= hi && k > cut.key) amount(k, &hist[bucket_of(k)]); },
-             [&](u64* hist) { cut_ties(lo, hi, bucket_of, hist); }, [&](u64) { return want; });
+      search(counting,
+             [&](uint32_t k) {
+               if (k < lo || k > hi || k <= cut.key) return;
+               if (counting) atomicAdd(&sh.counts[bucket_of(k)], 1u);
+               else if (const u64 f = w.fixed_of(k)) sh.add(bucket_of(k), f);
+             },
+             [&] {
+               if (!counting && cut.ties && cut.key >= lo && cut.key <= hi) sh.add(bucket_of(cut.key), w.fixed_of(cut.key) * cut.ties);
+             },
+             [&](u64) { return want; });
       wanted = sh.rest;
       const uint32_t b = sh.bucket, old = hi;
       hi = old - (b << shift);
       const uint32_t width = (1u << shift) - 1u;
       lo = max(lo, hi > width ? hi - width : 0u);
+      __syncthreads();                                   // (the found bucket has been read)
     }
-    *key = lo;
-    return wanted;
+    if (counting) return Cut{lo, (uint32_t)wanted};
+    const u64 each = w.fixed_of(lo);
+    u64 ties = each ? (wanted + each - 1) / each : 1ull;
+    if (lo == cut.key && ties > cut.ties) ties = cut.ties;
+    return Cut{lo, (uint32_t)min(max(ties, 1ull), 0xffffffffull)};
   };
 
   Cut cut{0u, 0u};
+  const float top_p = p.top_ps ? p.top_ps[row] : p.top_p;
+  auto nucleus = [&](u64 total) -> u64 { return (u64)ceil((double)fmaxf(top_p, 0.0f) * (double)total); };
   const int top_k = p.top_ks ? p.top_ks[row] : p.top_k;
   if (top_k > 0 && top_k < p.vocab) {
-    uint32_t key;
-    const u64 ties = threshold(value_of(low), true, Cut{0u, 0u}, [&](u64) { return (u64)top_k; }, &key);
-    cut = Cut{key, (uint32_t)ties};
+    const float sc = linear_of(value_of(low));
+    search(true, [&](uint32_t k) { if (k) atomicAdd(&sh.counts[linear(k, sc)], 1u); }, [] {}, [&](u64) { return (u64)top_k; });
+    if (sh.above + sh.in_bucket <= kMaxPairs) {
+      // few enough to finish on a list: ranks, the nucleus, and the draw in index order, by comparing all pairs
+      const uint32_t b0 = sh.bucket;
+      const int n = collect([&](uint32_t k) { return linear(k, sc) <= b0; });
+      if (rank == 0) {
+        const u64* all = sh.all_listed();
+        const u64 me = tid < n ? all[tid] : 0ull;
+        const uint32_t key = (uint32_t)(me >> 32);
+        const u64 mine = tid < n ? w.fixed_of(key) : 0ull;
+        if (tid < n) sh.pair_weight[tid] = mine;
+        __syncthreads();
+        u64 before = 0;
+        int ahead = 0;
+        if (tid < n)
+          for (int j = 0; j < n; ++j)
+            if (all[j] > me) { before += sh.pair_weight[j]; ++ahead; }
+        const bool ranked = tid < n && ahead < top_k;
+        auto block_sum = [&](u64 v) -> u64 {
+          v = warp_sum(v);
+          __syncthreads();
+          if (lane == 0) sh.warp_sum[warp] = v;
+          __syncthreads();
+          u64 s = 0;
+#pragma unroll
+          for (int i = 0; i < kMaxPairs / 32; ++i) s += sh.warp_sum[i];
+          return s;
+        };
+        const u64 reach = top_p < 1.0f ? nucleus(block_sum(ranked ? mine : 0ull)) : ~0ull;
+        const bool kept = ranked && (ahead == 0 || before < reach);
+        const u64 drawn = kept ? w.drawn(key) : 0ull;
+        const u64 total = block_sum(drawn);
+        if (tid < n) sh.pair_weight[tid] = drawn;
+        __syncthreads();
+        const u64 target = draw_target(total);
+        if (drawn) {
+          u64 run = 0;
+          for (int j = 0; j < n; ++j)
+            if ((uint32_t)all[j] > (uint32_t)me) run += sh.pair_weight[j];       // of lower index
+          if (run <= target && target < run + drawn) {
+            p.tokens[row] = (int64_t)(uint32_t)~(uint32_t)me;
+            if (p.probabilities) p.probabilities[row] = (float)(w.scaled(key) / (double)total);
+          }
+        }
+      }
+      cluster.sync();
+      return;
+    }
+    cut = resolve(sc, true, Cut{0u, 0u});
   }
-  const float top_p = p.top_ps ? p.top_ps[row] : p.top_p;
   if (top_p < 1.0f) {
-    uint32_t key;
-    const float reach = 34.0f * t;
-    const float x_low = fmaxf(value_of(low), w.top_value - reach);
-    const u64 weight = threshold(x_low, false, cut, [&](u64 total) { return (u64)ceil((double)fmaxf(top_p, 0.0f) * (double)total); }, &key);
-    const u64 each = w.fixed_of(key);
-    u64 ties = each ? (weight + each - 1) / each : 1ull;
-    if (ties < 1) ties = 1;
-    if (key == cut.key && ties > cut.ties) ties = cut.ties;
-    cut = Cut{key, (uint32_t)min(ties, 0xffffffffull)};
+    const float sc = linear_of(fmaxf(value_of(low), w.top_value - 34.0f * t));
+    const Cut by_rank = cut;
+    search(false,
+           [&](uint32_t k) {
+             const u64 f = w.fixed_of(k);
+             if (k <= by_rank.key || !f) return;
+             const uint32_t b = linear(k, sc);
+             sh.add(b, f);
+             atomicAdd(&sh.counts[b], 1u);
+           },
+           [&] { if (by_rank.ties) sh.add(linear(by_rank.key, sc), w.fixed_of(by_rank.key) * by_rank.ties); },
+           nucleus);
+    cut = resolve(sc, false, by_rank);
   }
 
   // ---- the draw: sums per warp segment in index order, then the segment, then the token ----
@@ -329,11 +509,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   {
     u64 sum = 0;
     uint32_t ties = 0;
+#pragma unroll 4
     for (int j = s0 + lane; j < s1; j += 32) {
       const uint32_t k = key_at(j);
-      if (k > cut.key) sum += w.drawn(k);
-      else if (k && k == cut.key) ++ties;
+      const u64 f = w.drawn(k);
+      sum += k > cut.key ? f : 0ull;
+      ties += k == cut.key;
     }
+    if (cut.key == 0u) ties = 0u;
     sum = warp_sum(sum);
     ties = __reduce_add_sync(0xffffffffu, ties);
     if (lane == 0) { sh.seg_sum[warp] = sum; sh.seg_ties[warp] = ties; }
@@ -360,10 +543,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     const u64 incl = warp_scan(mine, lane);
     const u64 total = __shfl_sync(0xffffffffu, incl, 31);
-    float u = p.uniforms[row];
-    u = u > 0.0f ? u : 0.0f;
-    u64 target = u < 1.0f ? (u64)((double)u * (double)total) : total;      // the running sum has to exceed this
-    if (target >= total) target = total - 1;
+    const u64 target = draw_target(total);
     const int at = __ffs(__ballot_sync(0xffffffffu, incl > target)) - 1;
     if (lane == at) {
       u64 before = incl - mine;
@@ -392,11 +572,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const int a0 = min(n, lane * per), a1 = min(n, a0 + per);
     u64 sum = 0;
     uint32_t ties = 0;
+#pragma unroll 4
     for (int j = a0; j < a1; ++j) {
       const uint32_t k = key_at(s0 + j);
-      if (k > cut.key) sum += w.drawn(k);
-      else if (k && k == cut.key) ++ties;
+      const u64 f = w.drawn(k);
+      sum += k > cut.key ? f : 0ull;
+      ties += k == cut.key;
     }
+    if (cut.key == 0u) ties = 0u;
     const uint32_t before = tb + (uint32_t)(warp_scan(ties, lane) - ties);
     const uint32_t left = cut.ties > before ? cut.ties - before : 0u;
     sum += tie_weight * (u64)min(ties, left);
@@ -417,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       if (hit) {
         if (lane == __ffs(hit) - 1) {
           p.tokens[row] = begin + s0 + j + lane;
-          if (p.probabilities) p.probabilities[row] = (float)(w.weight(k) * (double)(1ull << w.bits) / (double)sh.total);
+          if (p.probabilities) p.probabilities[row] = (float)(w.scaled(k) / (double)sh.total);
         }
         break;
       }
