@@ -52,7 +52,6 @@ constexpr uint32_t kLowestKey = 0x00800000u;           // of the lowest finite v
 // a weight below 2^-14 touches the upper word only with its carry.
 struct Shared {
   uint32_t low[kBuckets], high[kBuckets];
-  uint32_t counts[kBuckets];           // keys of each bucket
   u64 coarse[kCoarse];
   u64 listed[kMaxListed];              // this CTA's keys of a bucket: key << 32 | ~index, so that larger means ranked earlier
   u64 pair_weight[kMaxPairs];
@@ -64,8 +63,8 @@ struct Shared {
   uint32_t n_listed;
   // what one warp or thread found for all
   uint32_t all_top, all_bottom;
-  uint32_t bucket, in_bucket;
-  u64 above, total, rest;
+  uint32_t bucket;
+  u64 above, in_bucket, total, rest;
   int seg;
   uint32_t seg_tie_base;
   uint32_t cut_key, cut_ties;
@@ -76,6 +75,7 @@ struct Shared {
     const uint32_t h = (uint32_t)(f >> 32) + (old + v < old ? 1u : 0u);
     if (h) atomicAdd(&high[b], h);
   }
+  __device__ u64 sum(int b) const { return (u64)high[b] << 32 | low[b]; }
 };
 static_assert(kMaxListed * 8 <= 2 * kBuckets * 4, "the list fits where the sums were");
 
@@ -151,9 +151,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     return e >= 0 && e < p.vocab ? key_of(widen(x[e])) : 0u;
   };
 
+  // f(key, place in the slice) for [j0, j1), four at a time by `lanes` threads of which this is number `me`; j0 a multiple of four
+  auto each_key = [&](int j0, int j1, int me, int lanes, auto&& f) {
+#pragma unroll 2
+    for (int j = j0 + 4 * me; j < j1; j += 4 * lanes) {
+      uint4 k;
+      if (RES) k = *reinterpret_cast<const uint4*>(keys + j);
+      else k = make_uint4(key_at(j), key_at(j + 1), key_at(j + 2), key_at(j + 3));
+      f(k.x, j);
+      f(k.y, j + 1);
+      f(k.z, j + 2);
+      f(k.w, j + 3);
+    }
+  };
+
   // ---- read the slice; largest and smallest key ----
   uint32_t top = 0u, low = 0xffffffffu;
-  for (int i = tid; i < kBuckets; i += kThreads) { sh.low[i] = 0u; sh.high[i] = 0u; sh.counts[i] = 0u; }
+  for (int i = tid; i < kBuckets; i += kThreads) { sh.low[i] = 0u; sh.high[i] = 0u; }
   if (tid < 256) sh.table[tid] = exp2((double)tid / 256.0);
   if (tid == 0) sh.n_listed = 0u;
 #pragma unroll 4
@@ -246,23 +260,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   int round = 0;
   // One round: `add(key)` for this CTA's keys and `once()` for the cluster, then the bucket
   // in which the running sum (bucket 0 first) reaches the target.  target_of(total) gives the target from the round's
-  // total.  Counts are the sums of a round that counts.
-  auto search = [&](bool counting, auto&& add, auto&& once, auto&& target_of) {
+  // total.
+  auto search = [&](auto&& add, auto&& once, auto&& target_of) {
     if (round > 0) {
       cluster.sync();                        // the other CTAs have read the last round's
-      for (int i = tid; i < kBuckets; i += kThreads) { sh.low[i] = 0u; sh.high[i] = 0u; sh.counts[i] = 0u; }
+      for (int i = tid; i < kBuckets; i += kThreads) { sh.low[i] = 0u; sh.high[i] = 0u; }
       __syncthreads();
     }
     ++round;
     if (rank == 0 && tid == 0) once();
-#pragma unroll 4
-    for (int j = tid; j < slice; j += kThreads) add(key_at(j));
+    each_key(0, slice, tid, kThreads, [&](uint32_t k, int) { add(k); });
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kCoarse / kWarps; ++i) {
       const int c = warp + i * kWarps;
-      const int i32 = c * 32 + lane;
-      const u64 s = counting ? (u64)__reduce_add_sync(0xffffffffu, sh.counts[i32]) : warp_sum((u64)sh.high[i32] << 32 | sh.low[i32]);
+      const u64 s = warp_sum(sh.sum(c * 32 + lane));
       if (lane == 0) sh.coarse[c] = s;
     }
     cluster.sync();
@@ -286,15 +298,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       int c = 2 * at;
       if (above + a_at < target) { above += a_at; ++c; }
       u64 f = 0;
-      uint32_t n = 0;
 #pragma unroll
       for (int r = 0; r < kMaxCluster; ++r)
-        if (r < nc) {
-          const Shared* q = cluster.map_shared_rank(&sh, r);
-          if (!counting) f += (u64)q->high[c * 32 + lane] << 32 | q->low[c * 32 + lane];
-          n += q->counts[c * 32 + lane];
-        }
-      if (counting) f = n;
+        if (r < nc) f += cluster.map_shared_rank(&sh, r)->sum(c * 32 + lane);
       const u64 fi = warp_scan(f, lane);
       const int fl = __ffs(__ballot_sync(0xffffffffu, above + fi >= target)) - 1;
       if (lane == fl) {
@@ -302,32 +308,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         sh.above = above + fi - f;
         sh.total = total;
         sh.rest = target - (above + fi - f);       // how much of the bucket is wanted
-        sh.in_bucket = n;
+        sh.in_bucket = f;
       }
     }
     __syncthreads();
   };
-  // Collects the cluster's keys that `wanted` names (at most kMaxListed, the caller knows) into all_listed; returns their
-  // number.  `n_listed` is zero before; the lists may be read until the next cluster barrier.
-  auto collect = [&](auto&& wanted) -> int {
-    for (int j = tid; j < slice; j += kThreads) {
-      const uint32_t k = key_at(j);
+  // Collects the cluster's keys that `wanted` names into all_listed and returns their number; the list holds them when
+  // there are at most kMaxListed.  `n_listed` is zero before; the lists may be read until the next cluster barrier.
+  auto collect = [&](auto&& wanted) -> uint32_t {
+    each_key(0, slice, tid, kThreads, [&](uint32_t k, int j) {
       if (k && wanted(k)) {
         const uint32_t at = atomicAdd(&sh.n_listed, 1u);
         if (at < kMaxListed) sh.listed[at] = (u64)k << 32 | (uint32_t)~(uint32_t)(begin + j);
       }
-    }
+    });
     cluster.sync();
     u64* all = sh.all_listed();
-    uint32_t n = 0;
-    for (int r = 0; r < nc; ++r) {
-      const Shared* q = cluster.map_shared_rank(&sh, r);
-      const uint32_t m = q->n_listed;
-      for (uint32_t i = tid; i < m && n + i < kMaxListed; i += kThreads) all[n + i] = q->listed[i];
-      n += m;
+    uint32_t m[kMaxCluster], n = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) m[r] = r < nc ? cluster.map_shared_rank(&sh, r)->n_listed : 0u;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      for (uint32_t i = tid; i < m[r] && n + i < kMaxListed; i += kThreads) all[n + i] = cluster.map_shared_rank(&sh, r)->listed[i];
+      n += m[r];
     }
     __syncthreads();
-    return (int)min(n, (uint32_t)kMaxListed);
+    return n;
   };
   // The value at which the sum of what the kept keys count for (one, or their weights), largest first, reaches a target.
   auto linear_of = [&](float x_low) -> float {
@@ -343,22 +349,36 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   auto resolve = [&](float sc, bool counting, Cut cut) -> Cut {
     const uint32_t b0 = sh.bucket;
     u64 wanted = sh.rest;
-    const uint32_t held = sh.in_bucket;
     const bool splits_ties = !counting && cut.ties && linear(cut.key, sc) == b0;     // then the earlier cut's own ties are in it
-    if (held <= kMaxListed && !splits_ties) {
-      const int n = collect([&](uint32_t k) { return k > cut.key && linear(k, sc) == b0 && (counting || w.fixed_of(k)); });
+    // the bucket as a range of (top - value) sc, as linear() rounds it
+    const float v0 = b0 == 0u ? -CUDART_INF_F : (float)b0, v1 = b0 == kBuckets - 1u || sc == 0.0f ? CUDART_INF_F : (float)(b0 + 1u);
+    uint32_t held = kMaxListed + 1;
+    if (!splits_ties && (!counting || sh.in_bucket <= kMaxListed)) {
+      held = collect([&](uint32_t k) {
+        const float v = (w.top_value - value_of(k)) * sc;
+        return k > cut.key && !(v < v0) && !(v >= v1) && (counting || w.fixed_of(k));
+      });
+      if (held > kMaxListed) {
+        cluster.sync();                    // every count has been read
+        if (tid == 0) sh.n_listed = 0u;
+      }
+    }
+    if (held <= kMaxListed) {
+      const int n = (int)held;
       u64* all = sh.all_listed();
-      const int padded = n <= 1 ? 1 : 1 << (32 - __clz(n - 1));
+      const int log = n <= 1 ? 0 : 32 - __clz(n - 1), padded = 1 << log;
       for (int i = n + tid; i < padded; i += kThreads) all[i] = 0ull;
-      // bitonic, largest first
-      for (int size = 2; size <= padded; size *= 2)
-        for (int d = size / 2; d; d /= 2) {
-          __syncthreads();
+      __syncthreads();
+      // Bitonic, largest first; a thread takes pairs tid and tid + 512.  A warp's pairs less than 64 apart are its own.
+      for (int ls = 1; ls <= log; ++ls)
+        for (int ld = ls - 1; ld >= 0; --ld) {
           for (int i = tid; i < padded / 2; i += kThreads) {
-            const int x = (i / d) * 2 * d + i % d, y = x + d;
+            const int x = ((i >> ld) << (ld + 1)) | (i & ((1 << ld) - 1)), y = x + (1 << ld);
             const u64 p0 = all[x], p1 = all[y];
-            if ((p0 < p1) == ((x & size) == 0)) { all[x] = p1; all[y] = p0; }
+            if ((p0 < p1) == (((x >> ls) & 1) == 0)) { all[x] = p1; all[y] = p0; }
           }
+          if (ld > 5 || (ld == 0 && ls > 5)) __syncthreads();
+          else __syncwarp();
         }
       __syncthreads();
       // running sums of two neighbours a thread; the one that reaches what is wanted is the cut
@@ -406,10 +426,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       const int shift = max(0, 21 - __clz(hi - lo));     // 2048 buckets over the range
       auto bucket_of = [&](uint32_t k) { return (hi - k) >> shift; };
       const u64 want = wanted;
-      search(counting,
-             [&](uint32_t k) {
+      search([&](uint32_t k) {
                if (k < lo || k > hi || k <= cut.key) return;
-               if (counting) atomicAdd(&sh.counts[bucket_of(k)], 1u);
+               if (counting) atomicAdd(&sh.low[bucket_of(k)], 1u);
                else if (const u64 f = w.fixed_of(k)) sh.add(bucket_of(k), f);
              },
              [&] {
@@ -436,11 +455,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const int top_k = p.top_ks ? p.top_ks[row] : p.top_k;
   if (top_k > 0 && top_k < p.vocab) {
     const float sc = linear_of(value_of(low));
-    search(true, [&](uint32_t k) { if (k) atomicAdd(&sh.counts[linear(k, sc)], 1u); }, [] {}, [&](u64) { return (u64)top_k; });
+    search([&](uint32_t k) { if (k) atomicAdd(&sh.low[linear(k, sc)], 1u); }, [] {}, [&](u64) { return (u64)top_k; });
     if (sh.above + sh.in_bucket <= kMaxPairs) {
       // few enough to finish on a list: ranks, the nucleus, and the draw in index order, by comparing all pairs
       const uint32_t b0 = sh.bucket;
-      const int n = collect([&](uint32_t k) { return linear(k, sc) <= b0; });
+      const int n = (int)collect([&](uint32_t k) { return linear(k, sc) <= b0; });
       if (rank == 0) {
         const u64* all = sh.all_listed();
         const u64 me = tid < n ? all[tid] : 0ull;
@@ -489,13 +508,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (top_p < 1.0f) {
     const float sc = linear_of(fmaxf(value_of(low), w.top_value - 34.0f * t));
     const Cut by_rank = cut;
-    search(false,
-           [&](uint32_t k) {
+    search([&](uint32_t k) {
              const u64 f = w.fixed_of(k);
-             if (k <= by_rank.key || !f) return;
-             const uint32_t b = linear(k, sc);
-             sh.add(b, f);
-             atomicAdd(&sh.counts[b], 1u);
+             if (k > by_rank.key && f) sh.add(linear(k, sc), f);
            },
            [&] { if (by_rank.ties) sh.add(linear(by_rank.key, sc), w.fixed_of(by_rank.key) * by_rank.ties); },
            nucleus);
@@ -504,18 +519,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
   // ---- the draw: sums per warp segment in index order, then the segment, then the token ----
   const u64 tie_weight = cut.key ? w.drawn(cut.key) : 0ull;
-  const int seg_len = ((slice + kWarps * 32 - 1) / (kWarps * 32)) * 32;
+  const int seg_len = ((slice + kWarps * 128 - 1) / (kWarps * 128)) * 128;
   const int s0 = min(slice, warp * seg_len), s1 = min(slice, s0 + seg_len);
   {
     u64 sum = 0;
     uint32_t ties = 0;
-#pragma unroll 4
-    for (int j = s0 + lane; j < s1; j += 32) {
-      const uint32_t k = key_at(j);
+    each_key(s0, s1, lane, 32, [&](uint32_t k, int) {
       const u64 f = w.drawn(k);
       sum += k > cut.key ? f : 0ull;
       ties += k == cut.key;
-    }
+    });
     if (cut.key == 0u) ties = 0u;
     sum = warp_sum(sum);
     ties = __reduce_add_sync(0xffffffffu, ties);
@@ -523,23 +536,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   cluster.sync();
   if (warp == 0) {
-    // lane l holds the segments l * per ... of the cluster's nc * kWarps, in index order
-    const int n_seg = nc * kWarps, per = (n_seg + 31) / 32;
-    u64 mine = 0;
-    uint32_t ties = 0;
-    for (int i = 0; i < per; ++i) {
-      const int sg = lane * per + i;
-      if (sg < n_seg) ties += cluster.map_shared_rank(&sh, sg / kWarps)->seg_ties[sg % kWarps];
+    // lane l holds segments 4 l to 4 l + 3 of the cluster's, in index order
+    constexpr int PER = kMaxCluster * kWarps / 32;
+    u64 sums[PER], mine = 0;
+    uint32_t tied[PER], ties = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int sg = lane * PER + i;
+      const bool there = sg < nc * kWarps;
+      const Shared* r = cluster.map_shared_rank(&sh, there ? sg / kWarps : 0);
+      sums[i] = there ? r->seg_sum[sg % kWarps] : 0ull;
+      tied[i] = there ? r->seg_ties[sg % kWarps] : 0u;
     }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) ties += tied[i];
     const uint32_t ties_before = (uint32_t)(warp_scan(ties, lane) - ties);
     uint32_t tb = ties_before;
-    for (int i = 0; i < per; ++i) {
-      const int sg = lane * per + i;
-      if (sg >= n_seg) break;
-      const Shared* r = cluster.map_shared_rank(&sh, sg / kWarps);
-      const uint32_t n = r->seg_ties[sg % kWarps], left = cut.ties > tb ? cut.ties - tb : 0u;
-      mine += r->seg_sum[sg % kWarps] + tie_weight * (u64)min(n, left);
-      tb += n;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      sums[i] += tie_weight * (u64)min(tied[i], cut.ties > tb ? cut.ties - tb : 0u);
+      mine += sums[i];
+      tb += tied[i];
     }
     const u64 incl = warp_scan(mine, lane);
     const u64 total = __shfl_sync(0xffffffffu, incl, 31);
@@ -549,15 +566,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       u64 before = incl - mine;
       tb = ties_before;
       int found = -1;
-      for (int i = 0; i < per && found < 0; ++i) {
-        const int sg = lane * per + i;
-        if (sg >= n_seg) break;
-        const Shared* r = cluster.map_shared_rank(&sh, sg / kWarps);
-        const uint32_t n = r->seg_ties[sg % kWarps], left = cut.ties > tb ? cut.ties - tb : 0u;
-        const u64 here = r->seg_sum[sg % kWarps] + tie_weight * (u64)min(n, left);
-        if (before + here > target) found = sg;
-        else { before += here; tb += n; }
-      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (found < 0) {
+          if (before + sums[i] > target) found = lane * PER + i;
+          else { before += sums[i]; tb += tied[i]; }
+        }
       sh.seg = found;
       sh.rest = target - before;
       sh.seg_tie_base = tb;
