@@ -7,11 +7,11 @@
 // One generated token reads every key and value once and computes 4 D flops with each pair: the bound is memory, so the
 // layout serves the loads.  The query rows that share a key head (group x tokens) are the M rows of mma.sync tiles:
 // sixteen rows cost what one costs, and each key is read once for all of them.  tcgen05 has nothing to add here (its 128
-// rows would stand empty) and would need its operands in a swizzled layout.  A CTA's eight warps form 8 / RT groups; a
-// group owns RT 16-row tiles and walks its own key tiles through a ring of cp.async stages, synchronised by a barrier of
-// the group alone.  Groups keep a running maximum and sum in 32 bits and are joined in shared memory at the end; with
-// few rows the keys are also split over CTAs, whose partial results the last one to arrive joins in split order, so the
-// result does not depend on the order of arrival.
+// rows would stand empty) and would need its operands in a swizzled layout.  A CTA's warps form groups of RT; a group owns
+// RT 16-row tiles and walks its own key tiles through a ring of cp.async stages, synchronised by a barrier of the group
+// alone.  Groups keep a running maximum and sum in 32 bits and are joined in shared memory at the end; with few rows the
+// keys are also split over CTAs, whose partial results a second kernel joins in split order (a CTA per row: one CTA
+// joining 37 parts of 32 rows of 128 had taken 30 us).
 // fp32 operands are multiplied as three tf32 products (hi hi + hi lo + lo hi); each tile's P V starts from zero and is
 // added to O in registers, because the tensor core's own accumulation truncates.  16-bit P is rounded to the operand
 // type, half a step of 2^-9 (bf16) or 2^-12 (f16) that the final rounding of the result exceeds.
@@ -89,32 +89,32 @@ template <typename T> __device__ __forceinline__ float tanh_for(float x) {
 template <typename T, int DP_, int RT_>
 struct Cfg {
   static constexpr int DP = DP_, RT = RT_, ES = sizeof(T);
-  static constexpr int Warps = DP > 128 ? 4 : 8;
+  static constexpr int Warps = (RT == 4 && DP <= 128) || DP <= 64 ? 8 : 4;
+  static constexpr int PerSm = 2;                       // CTAs that share an SM (their start and end overlap)
   static constexpr int KG = Warps / RT;                 // key groups
   static constexpr int Threads = Warps * 32;
-  static constexpr int KT = ES == 2 ? (RT == 4 ? 32 : 16) : (RT == 1 ? 8 : 16);   // keys of a tile
+  static constexpr int KT = ES == 2 ? (RT == 1 ? 16 : 32) : (RT == 1 ? 8 : 16);   // keys of a tile
   static constexpr int LD = DP + 16 / ES;               // row stride in shared memory: 16 bytes of padding, no bank conflicts
   static constexpr int TileBytes = KT * LD * ES;        // one K or V tile
   static constexpr int SetBytes = KG * 2 * TileBytes;   // a stage of every group
   static constexpr int QBytes = 16 * RT * LD * ES;
-  static constexpr int Stages = RT == 4 ? 2 : (3 * SetBytes + QBytes <= 216 * 1024 ? 3 : 2);
+  static constexpr int Stages = RT == 4 ? 2 : (4 * SetBytes + QBytes <= 108 * 1024 ? 4 : 3 * SetBytes + QBytes <= 109 * 1024 ? 3 : 2);
   static constexpr int MergeLd = DP + 4;
   static constexpr int MergeBytes = Warps * 16 * MergeLd * 4;
   static constexpr int RingBytes = Stages * SetBytes;
   static constexpr int Smem = QBytes + (RingBytes > MergeBytes ? RingBytes : MergeBytes);
 };
-constexpr int kMaxSplits = 64;
 
 template <typename T, int DP, int RT>
-__global__ void __launch_bounds__(Cfg<T, DP, RT>::Threads, RT == 4 && DP <= 128 ? 2 : 1)
-cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, int row_tiles, int vec, float* partials, int* counters) {
+__global__ void __launch_bounds__(Cfg<T, DP, RT>::Threads, DP <= 128 ? 2 : 1)
+cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, int row_tiles, int vec, float* partials) {
   using C = Cfg<T, DP, RT>;
   constexpr int KT = C::KT, LD = C::LD, KG = C::KG, ST = C::Stages, ROWS = 16 * RT, GT = RT * 32;
   extern __shared__ __align__(128) unsigned char smem[];
   T* sQ = reinterpret_cast<T*>(smem);
   unsigned char* ring = smem + C::QBytes;
   __shared__ int s_hi[ROWS], s_pos[ROWS], s_doc[ROWS];
-  __shared__ int s_top, s_doc_min, s_doc_max, s_last;
+  __shared__ int s_top, s_doc_min, s_doc_max;
   __shared__ float s_m[C::Warps * 16], s_l[C::Warps * 16];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -125,9 +125,10 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
   const int bh = unit % n_bh, b = bh / p.hkv, hk = bh % p.hkv;
   const int n_rows = p.group * p.sq, row0 = row_tile * ROWS;
 
-  int len = p.sk;
+  // (all three requested before the first is used)
+  const int len_in = p.lengths ? __ldg(p.lengths + b) : p.sk, start_in = p.starts ? __ldg(p.starts + b) : 0, prefix = p.prefixes ? __ldg(p.prefixes + b) : 0;
+  int len = len_in;
   if (p.lengths) {
-    len = p.lengths[b];
     if (len < 0 || len > p.sk) {
       if (tid == 0) { *p.status.host = BG_ERR_INDEX_RANGE; *p.status.device = BG_ERR_INDEX_RANGE; }
       len = min(max(len, 0), p.sk);
@@ -141,9 +142,9 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
     int hi = 0, doc = -1;
     long long pos = 0;
     if (r < n_rows) {
-      pos = (p.starts ? (long long)p.starts[b] : (long long)len - p.sq) + r / p.group;
+      pos = (p.starts ? (long long)start_in : (long long)len - p.sq) + r / p.group;
       if (!p.causal) hi = len;
-      else if (pos >= 0 && pos < len) hi = min((long long)len, max(pos + 1, (long long)(p.prefixes ? p.prefixes[b] : 0)));
+      else if (pos >= 0 && pos < len) hi = min((long long)len, max(pos + 1, (long long)prefix));
       if (p.documents) {
         doc = pos >= 0 && pos < p.sk ? p.documents[(long long)b * p.sk + pos] : -1;
         if (doc < 0) hi = 0;
@@ -156,16 +157,6 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
       atomicMax(&s_top, hi);
       if (p.documents) { atomicMin(&s_doc_min, doc); atomicMax(&s_doc_max, doc); }
     }
-  }
-  // query rows -> shared memory, zeros where there is none
-  for (int i = tid; i < ROWS * DP; i += C::Threads) {
-    const int r = i / DP, d = i - r * DP;
-    T v = narrow<T>(0.0f);
-    if (row0 + r < n_rows && d < p.d) {
-      const int tok = (row0 + r) / p.group, g = (row0 + r) - tok * p.group;
-      v = reinterpret_cast<const T*>(p.q.ptr)[b * p.q.sb + tok * p.q.sr + (long long)(hk * p.group + g) * p.q.sh + d];
-    }
-    sQ[r * LD + d] = v;
   }
   __syncthreads();
 
@@ -192,7 +183,22 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
     T* dk = tile_ptr(stage, 0);
     T* dv = tile_ptr(stage, 1);
     constexpr int PER = 16 / C::ES, CPR = DP / PER;
-    if (vec) {
+    if ((vec & 1) && GT % CPR == 0) {
+      // a thread keeps its column and steps down the rows
+      const int r0 = gt / CPR, c = (gt - r0 * CPR) * PER;
+      constexpr int STEP = GT / CPR;
+      const T* ks = kp + (long long)(key0 + r0) * p.k.sr + c;
+      const T* vs = vp + (long long)(key0 + r0) * p.v.sr + c;
+      const int rows = c < p.d ? len - key0 - r0 : 0;          // of this column, counted from r0
+#pragma unroll
+      for (int r = 0; r < KT; r += STEP) {
+        const bool there = r < rows;
+        cp_async16(dk + (r0 + r) * LD + c, there ? ks : kp, there);
+        cp_async16(dv + (r0 + r) * LD + c, there ? vs : vp, there);
+        ks += STEP * p.k.sr;
+        vs += STEP * p.v.sr;
+      }
+    } else if (vec & 1) {
 #pragma unroll
       for (int i0 = 0; i0 < KT * CPR; i0 += GT) {
         const int i = i0 + gt;
@@ -229,24 +235,46 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
       if (row0 + ra + 8 * i < n_rows) slope_r[i] = p.slopes[hk * p.group + (row0 + ra + 8 * i) % p.group] * kLog2e;
   const float to_log2 = p.cap > 0.f ? p.cap * kLog2e : p.scale * kLog2e, to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f;
 
-  constexpr bool QREG = C::ES == 2 && DP <= 128;
-  uint32_t q_frag[QREG ? DP / 16 : 1][4];
-  if (QREG)
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) ldsm4(q_frag[QREG ? kk : 0], sQ + (rt * 16 + (lane & 15)) * LD + kk * 16 + (lane >> 4) * 8);
-
   float o[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   float m_r[2] = {-CUDART_INF_F, -CUDART_INF_F}, l_r[2] = {0.f, 0.f};
 
   int lt = next(t_begin + kg), ct = lt, issued = 0, done = 0;
+  // query rows -> shared memory, zeros where there is none; they arrive with the first key tile
+  if (vec & 2) {
+    constexpr int PER = 16 / C::ES, CPR = DP / PER;
+    for (int i = tid; i < ROWS * CPR; i += C::Threads) {
+      const int r = i / CPR, c = (i - r * CPR) * PER;
+      const bool there = row0 + r < n_rows && c < p.d;
+      const int row = there ? row0 + r : 0, tok = row / p.group, gh = row - tok * p.group;
+      cp_async16(sQ + r * LD + c, reinterpret_cast<const T*>(p.q.ptr) + b * p.q.sb + tok * p.q.sr + (long long)(hk * p.group + gh) * p.q.sh + (there ? c : 0), there);
+    }
+  } else {
+    for (int i = tid; i < ROWS * DP; i += C::Threads) {
+      const int r = i / DP, d = i - r * DP;
+      T v = narrow<T>(0.0f);
+      if (row0 + r < n_rows && d < p.d) {
+        const int tok = (row0 + r) / p.group, gh = (row0 + r) - tok * p.group;
+        v = reinterpret_cast<const T*>(p.q.ptr)[b * p.q.sb + tok * p.q.sr + (long long)(hk * p.group + gh) * p.q.sh + d];
+      }
+      sQ[r * LD + d] = v;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < ST - 1; ++i) {
     if (lt < t_end) { load(lt, issued % ST); lt = next(lt + KG); }
     ++issued;
     cp_async_commit();
   }
+  cp_async_wait<ST - 2>();
+  __syncthreads();
+  constexpr bool QREG = C::ES == 2 && DP <= 128;
+  uint32_t q_frag[QREG ? DP / 16 : 1][4];
+  if (QREG)
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) ldsm4(q_frag[QREG ? kk : 0], sQ + (rt * 16 + (lane & 15)) * LD + kk * 16 + (lane >> 4) * 8);
+
   while (ct < t_end) {
     cp_async_wait<ST - 2>();
     group_sync();
@@ -393,6 +421,7 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
     l_r[r] += __shfl_xor_sync(0xffffffffu, l_r[r], 2);
   }
   // ---- join the key groups: every warp leaves its 16 rows in shared memory ----
+  grid_launch_dependents();
   __syncthreads();
   float* mo = reinterpret_cast<float*>(ring) + warp * 16 * C::MergeLd;
 #pragma unroll
@@ -440,85 +469,96 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
       if (d == 0) { part[ROWS * DP + r] = m; part[ROWS * DP + ROWS + r] = l; }
     }
   }
-  if (!part) return;
-  // ---- join the splits: the CTA that arrives last reads all partial results, in split order ----
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    s_last = atomicAdd(counters + unit, 1) == splits - 1;
-    if (s_last) counters[unit] = 0;        // zero between launches
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  const float* all = partials + (long long)unit * splits * (ROWS * (DP + 2));
-  float* s_w = reinterpret_cast<float*>(ring);           // [splits][ROWS] weights of the partial results
-  for (int r = tid; r < live; r += C::Threads) {
-    float m = -CUDART_INF_F, l = 0.f;
-    for (int k = 0; k < splits; ++k) m = fmaxf(m, __ldcg(all + (long long)k * (ROWS * (DP + 2)) + ROWS * DP + r));
-    for (int k = 0; k < splits; ++k) {
-      const float* q = all + (long long)k * (ROWS * (DP + 2)) + ROWS * DP + r;
-      const float f = m == -CUDART_INF_F ? 0.f : ex2(__ldcg(q) - m);
-      s_w[k * ROWS + r] = f;
-      l = fmaf(f, __ldcg(q + ROWS), l);
-    }
-    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-    for (int k = 0; k < splits; ++k) s_w[k * ROWS + r] *= inv;
-  }
-  __syncthreads();
-  for (int i = tid; i < live * Q4; i += C::Threads) {
-    const int r = i / Q4, d = (i - r * Q4) * 4;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// Joins the parts of one row: four warps take the splits in turn, 16 bytes a lane.
+template <typename T, int DP, int RT>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ DecoderAttention p, int splits, int row_tiles, const float* partials) {
+  constexpr int ROWS = 16 * RT, STEP = ROWS * (DP + 2);
+  __shared__ float s_part[4][DP], s_sum[4];
+  grid_dependency_wait();
+  const int unit = blockIdx.x / ROWS, r = blockIdx.x % ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_bh = p.b * p.hkv, row_tile = row_tiles - 1 - unit / n_bh, bh = unit % n_bh, b = bh / p.hkv, hk = bh % p.hkv;
+  const int row = row_tile * ROWS + r;
+  if (row >= p.group * p.sq) return;
+  const float* all = partials + (long long)unit * splits * STEP;
+  float top = -CUDART_INF_F;
+  for (int k = lane; k < splits; k += 32) top = fmaxf(top, __ldg(all + (long long)k * STEP + ROWS * DP + r));
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  constexpr int PER = (DP + 127) / 128;
+  float4 acc[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  if (top != -CUDART_INF_F)
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(all + (long long)k * (ROWS * (DP + 2)) + r * DP + d));
-      const float f = s_w[k * ROWS + r];
-      a.x = fmaf(f, v.x, a.x); a.y = fmaf(f, v.y, a.y); a.z = fmaf(f, v.z, a.z); a.w = fmaf(f, v.w, a.w);
+    for (int k = warp; k < splits; k += 4) {
+      const float* q = all + (long long)k * STEP;
+      const float f = ex2(__ldg(q + ROWS * DP + r) - top);
+      sum = fmaf(f, __ldg(q + ROWS * DP + ROWS + r), sum);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int d = i * 128 + lane * 4;
+        if (d >= DP) continue;
+        const float4 v = __ldg(reinterpret_cast<const float4*>(q + r * DP + d));
+        acc[i].x = fmaf(f, v.x, acc[i].x); acc[i].y = fmaf(f, v.y, acc[i].y); acc[i].z = fmaf(f, v.z, acc[i].z); acc[i].w = fmaf(f, v.w, acc[i].w);
+      }
     }
-    store(r, d, a);
-  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (i * 128 + lane * 4 < DP) *reinterpret_cast<float4*>(&s_part[warp][i * 128 + lane * 4]) = acc[i];
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  const float l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  const int tok = row / p.group, gh = row - tok * p.group;
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + tok * p.out.sr + (long long)(hk * p.group + gh) * p.out.sh;
+  for (int d = threadIdx.x; d < p.d; d += 128) dst[d] = narrow<T>(((s_part[0][d] + s_part[1][d]) + (s_part[2][d] + s_part[3][d])) * inv);
 }
 
 template <typename T, int DP, int RT>
-cudaError_t launch_one(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, int* counters, cudaStream_t s) {
+cudaError_t launch_one(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s) {
   using C = Cfg<T, DP, RT>;
   static_assert(C::Smem + 4096 <= 227 * 1024, "shared memory of a CTA");
-  static_assert(kMaxSplits * 16 * RT * 4 <= C::Smem - C::QBytes, "split weights fit where the ring was");
   const int row_tiles = (p.group * p.sq + 16 * RT - 1) / (16 * RT);
   const long long grid = (long long)p.b * p.hkv * row_tiles * plan.splits;
   if (grid <= 0 || grid > 0x7fffffffll) return cudaErrorInvalidValue;
   constexpr int per = 16 / C::ES;
   const int vec = p.d % per == 0 && (reinterpret_cast<uintptr_t>(p.k.ptr) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.v.ptr) & 15) == 0 &&
-                  p.k.sr % per == 0 && p.v.sr % per == 0 && p.k.sb % per == 0 && p.v.sb % per == 0 && p.k.sh % per == 0 && p.v.sh % per == 0;
-  cudaError_t e = cudaFuncSetAttribute(cache_attention_kernel<T, DP, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::Smem);
+                  p.k.sr % per == 0 && p.v.sr % per == 0 && p.k.sb % per == 0 && p.v.sb % per == 0 && p.k.sh % per == 0 && p.v.sh % per == 0 ? 1 : 0;
+  const int qvec = p.d % per == 0 && (reinterpret_cast<uintptr_t>(p.q.ptr) & 15) == 0 && p.q.sr % per == 0 && p.q.sb % per == 0 && p.q.sh % per == 0 ? 2 : 0;
+  cudaError_t e = allow_shared(cache_attention_kernel<T, DP, RT>, C::Smem);
   if (e != cudaSuccess) return e;
-  cache_attention_kernel<T, DP, RT><<<(unsigned)grid, C::Threads, C::Smem, s>>>(p, plan.splits, row_tiles, vec, plan.splits > 1 ? partials : nullptr, counters);
-  return cudaGetLastError();
+  cache_attention_kernel<T, DP, RT><<<(unsigned)grid, C::Threads, C::Smem, s>>>(p, plan.splits, row_tiles, vec | qvec, plan.splits > 1 ? partials : nullptr);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || plan.splits == 1) return e;
+  return launch_dependent(join_kernel<T, DP, RT>, dim3((unsigned)(grid / plan.splits * 16 * RT)), dim3(128), 0, s, p, plan.splits, row_tiles, (const float*)partials);
 }
 
 template <typename T, int DP>
-cudaError_t launch_rows(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, int* counters, cudaStream_t s) {
-  return plan.row_tiles == 1 ? launch_one<T, DP, 1>(p, plan, partials, counters, s)
-         : plan.row_tiles == 2 ? launch_one<T, DP, 2>(p, plan, partials, counters, s) : launch_one<T, DP, 4>(p, plan, partials, counters, s);
+cudaError_t launch_rows(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s) {
+  return plan.row_tiles == 1 ? launch_one<T, DP, 1>(p, plan, partials, s)
+         : plan.row_tiles == 2 ? launch_one<T, DP, 2>(p, plan, partials, s) : launch_one<T, DP, 4>(p, plan, partials, s);
 }
 
 inline int padded_head(int d) { return d <= 64 ? 64 : d <= 80 ? 80 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
 
 template <typename T>
-cudaError_t launch_typed(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, int* counters, cudaStream_t s) {
+cudaError_t launch_typed(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s) {
   switch (padded_head(p.d)) {
-    case 64: return launch_rows<T, 64>(p, plan, partials, counters, s);
-    case 80: return launch_rows<T, 80>(p, plan, partials, counters, s);
-    case 96: return launch_rows<T, 96>(p, plan, partials, counters, s);
-    case 128: return launch_rows<T, 128>(p, plan, partials, counters, s);
-    default: return launch_rows<T, 256>(p, plan, partials, counters, s);
+    case 64: return launch_rows<T, 64>(p, plan, partials, s);
+    case 80: return launch_rows<T, 80>(p, plan, partials, s);
+    case 96: return launch_rows<T, 96>(p, plan, partials, s);
+    case 128: return launch_rows<T, 128>(p, plan, partials, s);
+    default: return launch_rows<T, 256>(p, plan, partials, s);
   }
 }
 
 // one translation unit per type
-cudaError_t launch_bf16(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, int* counters, cudaStream_t s);
-cudaError_t launch_f16(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, int* counters, cudaStream_t s);
-cudaError_t launch_f32(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, int* counters, cudaStream_t s);
+cudaError_t launch_bf16(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s);
+cudaError_t launch_f16(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s);
+cudaError_t launch_f32(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s);
 
 }  // namespace cache_attn
 }  // namespace bg

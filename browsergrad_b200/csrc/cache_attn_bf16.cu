@@ -3,8 +3,8 @@
 
 namespace bg {
 namespace cache_attn {
-cudaError_t launch_bf16(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, int* counters, cudaStream_t s) {
-  return launch_typed<__nv_bfloat16>(p, plan, partials, counters, s);
+cudaError_t launch_bf16(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s) {
+  return launch_typed<__nv_bfloat16>(p, plan, partials, s);
 }
 }  // namespace cache_attn
 }  // namespace bg

@@ -648,12 +648,13 @@ size_t smem_bytes(int sk) { return (size_t)Cfg<D>::Smem + 1024 + 256 + 2 * (size
 template <bool BF16, int D, bool CAP, bool BIAS>
 cudaError_t launch_kernel(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
   auto kern = prompt_attention_kernel<BF16, D, CAP, BIAS>;
-  cudaFuncAttributes fa;
-  cudaError_t e = cudaFuncGetAttributes(&fa, kern);
-  if (e != cudaSuccess) return e;
-  if (fa.numRegs < kLaunchRegs) return cudaErrorLaunchOutOfResources;
+  static const int regs = [&] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (regs < kLaunchRegs) return cudaErrorLaunchOutOfResources;
   const size_t smem = smem_bytes<D>(p.a.sk);
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_shared(kern, smem);
   if (e != cudaSuccess) return e;
   const int pairs = ((p.a.sq + kRows - 1) / kRows + 1) / 2;
   kern<<<(unsigned)((long long)pairs * p.a.b * p.a.hq), kThreads, smem, s>>>(q, k, v, p);

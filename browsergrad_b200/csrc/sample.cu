@@ -640,7 +640,7 @@ cudaError_t launch_typed(const SampleProblem& p, cudaStream_t s, int sm_count) {
   const bool res = slice <= room;
   void (*kern)(const SampleProblem, int) = res ? sample_kernel<T, true> : sample_kernel<T, false>;
   const size_t smem = fixed + (res ? (size_t)slice * 4 : 0);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_shared(kern, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   if (p.n * nc > 0x7fffffffll) return cudaErrorInvalidValue;

@@ -363,9 +363,7 @@ int decoder_attention(const Call& c, const bg_head_view* q, const bg_head_view* 
     if (plan.partial_bytes)
       if (int rc = partials.get(plan.partial_bytes)) return rc;
     const std::string name = std::string("cache_attention[") + dtype_name(dtype) + "] x" + std::to_string(plan.splits);
-    if (int rc = launch(c, name, 1, [&] {
-          return launch_cache_attention(p, dtype, plan, reinterpret_cast<float*>(partials.p), c.ctx->gemm_counters, c.ctx->stream);
-        })) return rc;
+    if (int rc = launch(c, name, plan.splits > 1 ? 2 : 1, [&] { return launch_cache_attention(p, dtype, plan, reinterpret_cast<float*>(partials.p), c.ctx->stream); })) return rc;
     c.ctx->status_pending = true;
   }
   *out = keep(&r, dtype, b, sq, hq, d);

@@ -17,6 +17,22 @@ struct StatusWords {
   int* host;
 };
 
+// Raises a kernel's limit of dynamic shared memory, once per kernel and device (the call costs about a microsecond).
+template <typename K>
+cudaError_t allow_shared(K kern, size_t bytes) {
+  struct Done { int device; size_t bytes; };
+  thread_local std::unordered_map<const void*, std::vector<Done>> done;      // a context is used from one thread at a time
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  auto& v = done[reinterpret_cast<const void*>(kern)];
+  for (auto& d : v)
+    if (d.device == dev && d.bytes >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) v.push_back({dev, bytes});
+  return e;
+}
+
 // ---- rotary.cu ---------------------------------------------------------------------------------------------------
 constexpr int kRotaryMaxPairs = 128;
 struct RotarySegment {
@@ -66,8 +82,7 @@ struct CacheAttnPlan {
   int64_t partial_bytes;
 };
 CacheAttnPlan cache_attention_plan(const DecoderAttention& p, int dtype, int sm_count);
-cudaError_t launch_cache_attention(const DecoderAttention& p, int dtype, const CacheAttnPlan& plan, float* partials, int* counters,
-                                   cudaStream_t s);
+cudaError_t launch_cache_attention(const DecoderAttention& p, int dtype, const CacheAttnPlan& plan, float* partials, cudaStream_t s);
 
 // Prompts of 16-bit operands (prompt_attn.cu).
 bool prompt_attention_usable(const DecoderAttention& p, int dtype);
