@@ -69,7 +69,7 @@ class HeadView(C.Structure):
     _fields_ = [("handle", C.c_int64), ("offset", C.c_int64), ("stride", C.c_int64 * 3)]
 
     def __init__(self, handle: int, strides: Sequence[int], offset: int = 0) -> None:
-        super().__init__(int(handle), int(offset), (C.c_int64 * 3)(*[int(v) for v in strides]))
+        super().__init__(handle, offset, tuple(strides))
 
     @classmethod
     def heads_first(cls, handle: int, rows: int, heads: int, dim: int) -> "HeadView":

@@ -32,13 +32,14 @@ struct alignas(VEC * sizeof(T)) Vec {
   T v[VEC];
 };
 
-// One item: the vectors at elements c * VEC of the first half and of the second half of the rotated part.
+// One item: the vectors at elements c * VEC of the first half and of the second half of the rotated part.  The sines and
+// cosines of a token lie so that threads of neighbouring c read neighbouring words: the i-th value of every item together.
 template <typename T, int VEC, bool INTER>
-__device__ __forceinline__ void turn_item(Vec<T, VEC>& lo, Vec<T, VEC>& hi, const float2* cs, int c, int half) {
+__device__ __forceinline__ void turn_item(Vec<T, VEC>& lo, Vec<T, VEC>& hi, const float2* cs, int c, int items) {
   if (!INTER) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const float2 w = cs[c * VEC + i];
+      const float2 w = cs[i * items + c];
       const float a = to_f(lo.v[i]), b = to_f(hi.v[i]);
       lo.v[i] = from_f<T>(a * w.x - b * w.y);
       hi.v[i] = from_f<T>(a * w.y + b * w.x);
@@ -46,7 +47,7 @@ __device__ __forceinline__ void turn_item(Vec<T, VEC>& lo, Vec<T, VEC>& hi, cons
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; i += 2) {
-      const float2 w = cs[(c * VEC + i) >> 1], z = cs[(half + c * VEC + i) >> 1];
+      const float2 w = cs[(i >> 1) * items + c], z = cs[((VEC + i) >> 1) * items + c];
       const float a = to_f(lo.v[i]), b = to_f(lo.v[i + 1]), e = to_f(hi.v[i]), f = to_f(hi.v[i + 1]);
       lo.v[i] = from_f<T>(a * w.x - b * w.y);
       lo.v[i + 1] = from_f<T>(a * w.y + b * w.x);
@@ -54,6 +55,16 @@ __device__ __forceinline__ void turn_item(Vec<T, VEC>& lo, Vec<T, VEC>& hi, cons
       hi.v[i + 1] = from_f<T>(e * z.y + f * z.x);
     }
   }
+}
+// Where turn_item looks for pair j's sine and cosine.
+template <int VEC, bool INTER>
+__device__ __forceinline__ int place_of(int j, int half) {
+  const int items = half / VEC;
+  if (VEC == 1) return j;
+  if (!INTER) return (j % VEC) * items + j / VEC;
+  constexpr int PER = VEC / 2 > 0 ? VEC / 2 : 1;          // pairs of one vector
+  const int second = j >= half / 2 ? 1 : 0, q = j - second * (half / 2);
+  return (second * PER + q % PER) * items + q / PER;
 }
 
 // VEC = 1 handles what vectors cannot: odd sizes, strides or addresses that are not multiples of a vector.  An item is
@@ -66,15 +77,6 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const int n_tok = min(tokens_per_cta, p.s - s0);
   const int half = p.rot >> 1;
   const int64_t first = p.starts ? (int64_t)p.starts[batch] : p.start;
-  for (int i = threadIdx.x; i < n_tok * half; i += kThreads) {
-    const int tok = i / half, j = i - tok * half;
-    const int64_t at = p.positions ? (int64_t)p.positions[(int64_t)batch * p.s + s0 + tok] : first + s0 + tok;
-    const double turns = (double)at * p.turns[j];
-    const float frac = (float)(turns - rint(turns));
-    float sn, cs;
-    sincospif(2.0f * frac, &sn, &cs);
-    s_cs[i] = make_float2(cs * p.magnitude, sn * p.magnitude);
-  }
   int64_t count = p.s;
   if (p.counts) {
     count = p.counts[batch];
@@ -83,44 +85,59 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
       count = count < 0 ? 0 : p.s;
     }
   }
+  for (int i = threadIdx.x; i < n_tok * half; i += kThreads) {
+    const int tok = i / half, j = i - tok * half;
+    const int64_t at = p.positions ? (int64_t)p.positions[(int64_t)batch * p.s + s0 + tok] : first + s0 + tok;
+    const double turns = (double)at * p.turns[j];
+    const float frac = (float)(turns - rint(turns));
+    float sn, cs;
+    sincospif(2.0f * frac, &sn, &cs);
+    s_cs[tok * half + place_of<VEC, INTER>(j, half)] = make_float2(cs * p.magnitude, sn * p.magnitude);
+  }
   __syncthreads();
-  const int pairs = half / VEC;                 // items of the rotated part (two vectors each)
-  const int rest = (p.d - p.rot) / VEC;         // vectors behind it
-  const int per_head = pairs + rest;
+  // items of a head: those of the rotated part, then the values behind it, two vectors an item
+  const int pairs = half / VEC, rest = (p.d - p.rot) / VEC, rest_items = (rest + 1) / 2;
+  const int per_head = pairs + rest_items;
   int h_total = 0;
   for (int g = 0; g < p.n_seg; ++g) h_total += p.seg[g].heads;
-  const int items = n_tok * h_total * per_head;
   using V = Vec<T, VEC>;
-  for (int it = threadIdx.x; it < items; it += kThreads) {
-    const int c = it % per_head;
-    int head = (it / per_head) % h_total;
-    const int tok = it / (per_head * h_total);
-    int g = 0;
-    while (head >= p.seg[g].heads) head -= p.seg[g++].heads;
+  // (c, head, tok) of this thread's items, advanced without divisions
+  const int dc = kThreads % per_head, dh = (kThreads / per_head) % h_total, dt = kThreads / per_head / h_total;
+  int c = threadIdx.x % per_head, head = (int)threadIdx.x / per_head % h_total, tok = (int)threadIdx.x / per_head / h_total;
+  while (tok < n_tok) {
+    int h = head, g = 0;
+    while (h >= p.seg[g].heads) h -= p.seg[g++].heads;
     const RotarySegment& sg = p.seg[g];
     int64_t row_out = s0 + tok;
+    bool keep = true;
     if (sg.cached) {
-      if (s0 + tok >= count) continue;
+      keep = s0 + tok < count;
       row_out += first;
-      if (row_out < 0 || row_out >= p.capacity) {
+      if (keep && (row_out < 0 || row_out >= p.capacity)) {
         *p.status.host = BG_ERR_INDEX_RANGE;
         *p.status.device = BG_ERR_INDEX_RANGE;
-        continue;
+        keep = false;
       }
     }
-    const T* x = reinterpret_cast<const T*>(sg.in.ptr) + batch * sg.in.sb + (int64_t)(s0 + tok) * sg.in.sr + head * sg.in.sh;
-    T* y = reinterpret_cast<T*>(const_cast<void*>(sg.out.ptr)) + batch * sg.out.sb + row_out * sg.out.sr + head * sg.out.sh;
-    if (c < pairs) {
-      const int e0 = VEC == 1 && INTER ? 2 * c : c * VEC;
-      const int e1 = VEC == 1 && INTER ? 2 * c + 1 : half + c * VEC;
-      V lo = *reinterpret_cast<const V*>(x + e0), hi = *reinterpret_cast<const V*>(x + e1);
-      if (sg.turn) turn_item<T, VEC, INTER && VEC != 1>(lo, hi, s_cs + tok * half, c, half);
+    if (keep) {
+      const T* x = reinterpret_cast<const T*>(sg.in.ptr) + batch * sg.in.sb + (int64_t)(s0 + tok) * sg.in.sr + h * sg.in.sh;
+      T* y = reinterpret_cast<T*>(const_cast<void*>(sg.out.ptr)) + batch * sg.out.sb + row_out * sg.out.sr + h * sg.out.sh;
+      const bool turned = c < pairs;
+      const int k = c - pairs;
+      const int e0 = turned ? (VEC == 1 && INTER ? 2 * c : c * VEC) : p.rot + k * VEC;
+      const int e1 = turned ? (VEC == 1 && INTER ? 2 * c + 1 : half + c * VEC) : p.rot + (k + rest_items) * VEC;
+      const bool both = turned || k + rest_items < rest;
+      V lo = *reinterpret_cast<const V*>(x + e0), hi = lo;
+      if (both) hi = *reinterpret_cast<const V*>(x + e1);
+      if (turned && sg.turn) turn_item<T, VEC, INTER && VEC != 1>(lo, hi, s_cs + tok * half, c, pairs);
       *reinterpret_cast<V*>(y + e0) = lo;
-      *reinterpret_cast<V*>(y + e1) = hi;
-    } else {
-      const int e = p.rot + (c - pairs) * VEC;
-      *reinterpret_cast<V*>(y + e) = *reinterpret_cast<const V*>(x + e);
+      if (both) *reinterpret_cast<V*>(y + e1) = hi;
     }
+    c += dc;
+    head += dh;
+    tok += dt;
+    if (c >= per_head) { c -= per_head; ++head; }
+    if (head >= h_total) { head -= h_total; ++tok; }
   }
 }
 
@@ -128,7 +145,7 @@ template <typename T, int VEC>
 cudaError_t launch_vec(const RotaryProblem& p, cudaStream_t s) {
   int heads = 0;
   for (int g = 0; g < p.n_seg; ++g) heads += p.seg[g].heads;
-  const int per_token = heads * (p.rot / 2 / VEC + (p.d - p.rot) / VEC);
+  const int per_token = heads * (p.rot / 2 / VEC + ((p.d - p.rot) / VEC + 1) / 2);
   // four items a thread: enough loads in flight without emptying the grid
   int tok = (4 * kThreads + per_token - 1) / per_token;
   if (tok > kMaxTokens) tok = kMaxTokens;
