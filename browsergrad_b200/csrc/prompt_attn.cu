@@ -26,12 +26,14 @@
 #include <math_constants.h>
 
 #include "attn_common.cuh"
+#include "prompt_common.cuh"
 #include "tc_common.cuh"
 
 namespace bg {
 namespace {
 
 using namespace tc;
+using namespace prompt;
 using attn::ex2_approx;
 using attn::fmax3;
 using attn::tma_load_4d;
@@ -39,7 +41,6 @@ using attn::tma_load_4d;
 constexpr int kRows = 128, kKeys = 128, kThreads = 384;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyLog2 = 8.0f;
-constexpr int kMaxPos = 1 << 30;
 // Registers move from warps 0-3 to the softmax warps: (128 x 72 + 256 x 216) / 384 = 168 a thread, what the CTA is
 // launched with (checked at launch; a request beyond the pool would wait for ever).
 constexpr int kLaunchRegs = 168, kLightRegs = 72, kSoftmaxRegs = 216;
@@ -103,24 +104,6 @@ __device__ __noinline__ uint32_t hide_scores(uint32_t t_s, uint4 seen) {
   tmem_st_wait();
   return (w[0] == 0u ? 1u : 0u) | (w[1] == 0u ? 2u : 0u) | (w[2] == 0u ? 4u : 0u) | (w[3] == 0u ? 8u : 0u);
 }
-// Bits of the keys (of `keys` that exist from docs on) whose document is this lane's.  Each key's id is read once per warp;
-// the rows of a warp belong to few documents, so the words are made per document, by ballots, not per row.
-__device__ __noinline__ uint4 document_bits(const int* docs, int keys, int doc) {
-  const int lane = threadIdx.x & 31;
-  int id[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) id[c] = c * 32 + lane < keys ? __ldg(docs + c * 32 + lane) : -1;
-  uint4 w = make_uint4(0u, 0u, 0u, 0u);
-  uint32_t left = __ballot_sync(0xffffffffu, doc >= 0);
-  while (left) {
-    const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
-    const uint4 v = make_uint4(__ballot_sync(0xffffffffu, id[0] == d), __ballot_sync(0xffffffffu, id[1] == d),
-                               __ballot_sync(0xffffffffu, id[2] == d), __ballot_sync(0xffffffffu, id[3] == d));
-    if (doc == d) w = v;
-    left &= ~__ballot_sync(0xffffffffu, doc == d);
-  }
-  return w;
-}
 template <int D>
 __device__ __noinline__ void rescale_row(uint32_t t_o, float alpha) {
 #pragma unroll 1
@@ -131,24 +114,6 @@ __device__ __noinline__ void rescale_row(uint32_t t_o, float alpha) {
     for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
     tmem_st32(t_o + (uint32_t)(c * 32), r);
   }
-}
-
-// Rows [i0, i1] of sequence b: the positions among them that see any key, and how many keys the last of them sees.
-struct Reach {
-  int first, last, keys;       // first > last: none
-};
-__device__ __forceinline__ Reach reach_of(const DecoderAttention& a, int b, int len, int i0, int i1) {
-  const long long start = a.starts ? (long long)a.starts[b] : (long long)len - a.sq;
-  long long p0 = start + i0, p1 = start + i1;
-  if (!a.causal) {
-    p0 = min(max(p0, (long long)-kMaxPos), (long long)kMaxPos);
-    p1 = min(max(p1, (long long)-kMaxPos), (long long)kMaxPos);
-    return Reach{(int)p0, (int)p1, i0 <= i1 ? len : 0};
-  }
-  p0 = max(p0, 0ll);
-  p1 = min(p1, (long long)len - 1);
-  if (i0 > i1 || p0 > p1) return Reach{1, 0, 0};
-  return Reach{(int)p0, (int)p1, (int)min((long long)len, max(p1 + 1, (long long)(a.prefixes ? a.prefixes[b] : 0)))};
 }
 
 template <bool BF16, int D, bool CAP, bool BIAS>
@@ -187,39 +152,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const int b = bh / a.hq, h = bh % a.hq, hk = h / a.group;
   const bool has_b = 2 * pair + 1 < n_qt;
 
-  int len = a.sk;
-  if (a.lengths) {
-    len = a.lengths[b];
-    if (len < 0 || len > a.sk) {
-      if (threadIdx.x == 0) { *a.status.host = BG_ERR_INDEX_RANGE; *a.status.device = BG_ERR_INDEX_RANGE; }
-      len = min(max(len, 0), a.sk);
-    }
-  }
+  const int len = length_of(a, b);
   const int n_kv = (len + kKeys - 1) / kKeys;
   const int2* ranges = a.documents ? a.doc_ranges + (long long)b * ((a.sk + kDocBlock - 1) / kDocBlock) : nullptr;
   const int* docs = a.documents ? a.documents + (long long)b * a.sk : nullptr;
-  // which key tiles each query tile needs
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int i0 = (2 * pair + g) * kRows, i1 = min(i0 + kRows, a.sq) - 1;
-    const Reach r = reach_of(a, b, len, i0, i1);
-    int doc_lo = INT_MAX, doc_hi = -1;
-    if (ranges)
-      for (int t = max(r.first, 0) / kDocBlock; t <= min(r.last, a.sk - 1) / kDocBlock && r.first <= r.last && r.last >= 0; ++t) {
-        const int2 x = __ldg(ranges + t);
-        doc_lo = min(doc_lo, x.x & 0x7fffffff);
-        doc_hi = max(doc_hi, x.y);
-      }
-    const int end = (r.keys + kKeys - 1) / kKeys;
-    for (int j = threadIdx.x; j < n_kv; j += kThreads) {
-      bool need = j < end;
-      if (need && ranges) {
-        const int2 x = __ldg(ranges + j);
-        need = (x.x & 0x7fffffff) <= doc_hi && x.y >= doc_lo;
-      }
-      s_need[g * n_kv + j] = need;
-    }
-  }
+  for (int g = 0; g < 2; ++g)
+    needed_tiles<kKeys>(a, b, len, (2 * pair + g) * kRows, min((2 * pair + g + 1) * kRows, a.sq) - 1, s_need + g * n_kv, threadIdx.x, kThreads);
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
       mbar_init(&q_full[g], 1);
@@ -603,45 +542,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   }
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult qr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess)
-      return reinterpret_cast<EncodeTiledFn>(p);
-    cudaGetLastError();
-    return (EncodeTiledFn) nullptr;
-  }();
-  return fn;
-}
-
-// Boxes of 128 rows x 64 values with the 128-byte swizzle; values behind d and rows behind the last arrive as zeros.
-bool make_map(CUtensorMap* map, const HeadPtr& v, int dtype, int b, int rows, int heads, int d) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
-  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)b};
-  // an axis of extent one has no stride: any legal value will do
-  const cuuint64_t any = ((cuuint64_t)d * 2 + 15) / 16 * 16;
-  cuuint64_t strides[3] = {rows > 1 ? (cuuint64_t)v.sr * 2 : any, heads > 1 ? (cuuint64_t)v.sh * 2 : any, b > 1 ? (cuuint64_t)v.sb * 2 : any};
-  cuuint32_t box[4] = {64, 128, 1, 1}, step[4] = {1, 1, 1, 1};
-  return fn(map, dtype == BG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(v.ptr), dims, strides,
-            box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// What TMA asks of a view: 16-byte steps below 2^40 bytes, no axis that stands still.
-bool view_fits(const HeadPtr& v, int b, int rows, int heads) {
-  if (reinterpret_cast<uintptr_t>(v.ptr) & 15) return false;
-  const int64_t st[3] = {v.sr, v.sh, v.sb};
-  const int ext[3] = {rows, heads, b};
-  for (int i = 0; i < 3; ++i)
-    if (ext[i] > 1 && (st[i] <= 0 || st[i] % 8 || st[i] >= ((int64_t)1 << 38))) return false;
-  return true;
-}
-
 template <int D>
 size_t smem_bytes(int sk) { return (size_t)Cfg<D>::Smem + 1024 + 256 + 2 * (size_t)((sk + kKeys - 1) / kKeys); }
 
@@ -672,18 +572,20 @@ cudaError_t launch_rules(const PromptParams& p, const CUtensorMap& q, const CUte
 }  // namespace
 
 bool prompt_attention_usable(const DecoderAttention& p, int dtype) {
+  if (dtype == BG_F32) return prompt_attention32_usable(p);
   if ((dtype != BG_BF16 && dtype != BG_F16) || p.d > 128 || p.d % 8 || p.sk == 0 || !encode_fn()) return false;
   // Below 64 rows a head most of a 128-row tile would stand empty, and the key-split kernel reads each key once for the
   // whole group.
   if (p.sq < 64) return false;
   if (smem_bytes<128>(p.sk) > 227 * 1024) return false;
   if ((long long)((p.sq + 255) / 256) * p.b * p.hq > 0x7fffffffll) return false;
-  return view_fits(p.q, p.b, p.sq, p.hq) && view_fits(p.k, p.b, p.sk, p.hkv) && view_fits(p.v, p.b, p.sk, p.hkv) && view_fits(p.out, p.b, p.sq, p.hq);
+  return view_fits(p.q, dtype, p.b, p.sq, p.hq) && view_fits(p.k, dtype, p.b, p.sk, p.hkv) && view_fits(p.v, dtype, p.b, p.sk, p.hkv) && view_fits(p.out, dtype, p.b, p.sq, p.hq);
 }
 
 cudaError_t launch_prompt_attention(const DecoderAttention& p, int dtype, cudaStream_t s) {
+  if (dtype == BG_F32) return launch_prompt_attention32(p, s);
   CUtensorMap q, k, v;
-  if (!make_map(&q, p.q, dtype, p.b, p.sq, p.hq, p.d) || !make_map(&k, p.k, dtype, p.b, p.sk, p.hkv, p.d) || !make_map(&v, p.v, dtype, p.b, p.sk, p.hkv, p.d))
+  if (!make_map(&q, p.q, dtype, p.b, p.sq, p.hq, p.d, kRows) || !make_map(&k, p.k, dtype, p.b, p.sk, p.hkv, p.d, kKeys) || !make_map(&v, p.v, dtype, p.b, p.sk, p.hkv, p.d, kKeys))
     return cudaErrorInvalidValue;
   const bool bf = dtype == BG_BF16, wide = p.d > 64;
   const uint32_t fmt = bf ? 1u : 0u;
