@@ -13,7 +13,8 @@
 // scores it was made from, and the next scores wait for P V.  The reference of the exponentials follows the row maximum
 // lazily: O is rescaled when the maximum has grown by more than 2^8.
 // Which keys a row sees is one number, the end of its visible range, and for packed documents the row's id: tiles nobody
-// sees are not loaded, tiles everybody sees are not masked, the rest are masked in tensor memory away from the main path.
+// sees are not loaded, tiles everybody sees are not masked, for the rest the bits of the keys seen are made while the
+// tile's scores are (a pass over the scores in tensor memory, kept out of the main path, had cost 1600 clocks a tile).
 // Bound: 4 D flops a visible pair on the tensor pipe (1024 clocks a tile of 128 x 128 x 128) against one exponential a
 // pair on the MUFU (16 a clock: 1024 clocks).  A cap would add two more MUFU operations; within |s| <= cap, where scores
 // nearly always lie, tanh is an odd polynomial on the FMA pipe instead, two values an instruction.
@@ -85,25 +86,6 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b, float
 
 // ---- rare work, out of the main path ----
 
-// Replaces the scores of this thread's row that are not seen by -inf; returns a bit per 32 keys none of which is seen.
-__device__ __noinline__ uint32_t hide_scores(uint32_t t_s, uint4 seen) {
-  uint32_t r[128];
-  tmem_ld32_issue(t_s, r);
-  tmem_ld32_issue(t_s + 32, r + 32);
-  tmem_ld32_issue(t_s + 64, r + 64);
-  tmem_ld32_issue(t_s + 96, r + 96);
-  tmem_ld_wait();
-  const uint32_t w[4] = {seen.x, seen.y, seen.z, seen.w};
-#pragma unroll
-  for (int i = 0; i < 128; ++i)
-    if (!((w[i >> 5] >> (i & 31)) & 1u)) r[i] = __float_as_uint(-CUDART_INF_F);
-  tmem_st32_issue(t_s, r);
-  tmem_st32_issue(t_s + 32, r + 32);
-  tmem_st32_issue(t_s + 64, r + 64);
-  tmem_st32_issue(t_s + 96, r + 96);
-  tmem_st_wait();
-  return (w[0] == 0u ? 1u : 0u) | (w[1] == 0u ? 2u : 0u) | (w[2] == 0u ? 4u : 0u) | (w[3] == 0u ? 8u : 0u);
-}
 template <int D>
 __device__ __noinline__ void rescale_row(uint32_t t_o, float alpha) {
 #pragma unroll 1
@@ -152,13 +134,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const int b = bh / a.hq, h = bh % a.hq, hk = h / a.group;
   const bool has_b = 2 * pair + 1 < n_qt;
 
-  const int len = length_of(a, b);
+  const Sequence seq = sequence_of(a, b);
+  const int len = seq.len;
   const int n_kv = (len + kKeys - 1) / kKeys;
   const int2* ranges = a.documents ? a.doc_ranges + (long long)b * ((a.sk + kDocBlock - 1) / kDocBlock) : nullptr;
   const int* docs = a.documents ? a.documents + (long long)b * a.sk : nullptr;
 #pragma unroll
   for (int g = 0; g < 2; ++g)
-    needed_tiles<kKeys>(a, b, len, (2 * pair + g) * kRows, min((2 * pair + g + 1) * kRows, a.sq) - 1, s_need + g * n_kv, threadIdx.x, kThreads);
+    needed_tiles<kKeys>(a, b, seq, (2 * pair + g) * kRows, min((2 * pair + g + 1) * kRows, a.sq) - 1, s_need + g * n_kv, threadIdx.x, kThreads);
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
       mbar_init(&q_full[g], 1);
@@ -318,7 +301,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const uint32_t t_o = tmem_base + (uint32_t)(C::ColO + g * D) + lane_sel;
       const uint32_t t_p = tmem_base + (uint32_t)(C::ColP + g * C::StepP) + lane_sel;
       const unsigned char* need = s_need + g * n_kv;
-      const Reach me = reach_of(a, b, len, row, row_ok ? row : row - 1);
+      const Reach me = reach_of(a, seq, row, row_ok ? row : row - 1);
       int hi = me.keys, doc = -1;
       if (docs) {
         doc = me.keys > 0 && me.first >= 0 && me.first < a.sk ? __ldg(docs + me.first) : -1;
@@ -342,6 +325,17 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           whole = whole && x.x == doc && x.y == doc;      // a block with keys of no document has its sign bit set
         }
         const bool hide = !__all_sync(0xffffffffu, whole);
+        // the bits of the keys seen, made while the scores are (warp-uniform; all set where nothing is hidden)
+        uint32_t seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (hide) {
+          const int n = min(max(hi - k0, 0), kKeys);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) seen[c] = n >= 32 * c + 32 ? 0xffffffffu : n <= 32 * c ? 0u : (1u << (n - 32 * c)) - 1u;
+          if (docs) {
+            const uint4 mine = document_bits(docs + k0, min(a.sk - k0, kKeys), doc);
+            seen[0] &= mine.x; seen[1] &= mine.y; seen[2] &= mine.z; seen[3] &= mine.w;
+          }
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g], (uint32_t)t & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after();
@@ -397,26 +391,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         }
         uint32_t dead = 0u;                                 // 32-key pieces that no row of this warp sees
         if (hide) {
-          tmem_st32_issue(t_s, xu);
-          tmem_st32_issue(t_s + 32, xu + 32);
-          tmem_st32_issue(t_s + 64, xu + 64);
-          tmem_st32_issue(t_s + 96, xu + 96);
-          tmem_st_wait();
-          const int n = min(max(hi - k0, 0), kKeys);
-          uint32_t w[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) w[c] = n >= 32 * c + 32 ? 0xffffffffu : n <= 32 * c ? 0u : (1u << (n - 32 * c)) - 1u;
-          uint4 seen = make_uint4(w[0], w[1], w[2], w[3]);
-          if (docs) {
-            const uint4 mine = document_bits(docs + k0, min(a.sk - k0, kKeys), doc);
-            seen = make_uint4(seen.x & mine.x, seen.y & mine.y, seen.z & mine.z, seen.w & mine.w);
-          }
-          dead = __reduce_and_sync(0xffffffffu, hide_scores(t_s, seen));
-          tmem_ld32_issue(t_s, xu);
-          tmem_ld32_issue(t_s + 32, xu + 32);
-          tmem_ld32_issue(t_s + 64, xu + 64);
-          tmem_ld32_issue(t_s + 96, xu + 96);
-          tmem_ld_wait();
+          for (int i = 0; i < kKeys; ++i)
+            if (!((seen[i >> 5] >> (i & 31)) & 1u)) x[i] = -CUDART_INF_F;
+          dead = __reduce_and_sync(0xffffffffu, (seen[0] == 0u ? 1u : 0u) | (seen[1] == 0u ? 2u : 0u) | (seen[2] == 0u ? 4u : 0u) | (seen[3] == 0u ? 8u : 0u));
         }
         if (!C::Alias) {
           tc_fence_before();

@@ -128,11 +128,12 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
   const int bh = (int)(blockIdx.x % (unsigned)n_bh);
   const int b = bh / a.hq, h = bh % a.hq, hk = h / a.group;
   const int q0 = q_tile * kRows;
-  const int len = length_of(a, b);
+  const Sequence seq = sequence_of(a, b);
+  const int len = seq.len;
   const int n_kv = (len + kKeys - 1) / kKeys;
   const int2* ranges = a.documents ? a.doc_ranges + (long long)b * ((a.sk + kDocBlock - 1) / kDocBlock) : nullptr;
   const int* docs = a.documents ? a.documents + (long long)b * a.sk : nullptr;
-  needed_tiles<kKeys>(a, b, len, q0, min(q0 + kRows, a.sq) - 1, s_need, threadIdx.x, kThreads);
+  needed_tiles<kKeys>(a, b, seq, q0, min(q0 + kRows, a.sq) - 1, s_need, threadIdx.x, kThreads);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 4);
     mbar_init(q_raw, 1);
@@ -278,7 +279,7 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
 #pragma unroll
     for (int d = 0; d < kDim; ++d) o[d] = 0.f;
     float m_ref = -CUDART_INF_F, l = 0.f;            // in powers of two
-    const Reach me = reach_of(a, b, len, row, row_ok ? row : row - 1);
+    const Reach me = reach_of(a, seq, row, row_ok ? row : row - 1);
     int hi = me.keys, doc = -1;
     if (docs) {
       doc = me.keys > 0 && me.first >= 0 && me.first < a.sk ? __ldg(docs + me.first) : -1;
@@ -310,6 +311,17 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         whole = whole && x.x == doc && x.y == doc;
       }
       const bool hide = !__all_sync(0xffffffffu, whole);
+      uint32_t w[2] = {0xffffffffu, 0xffffffffu};         // the keys seen, made while the scores are
+      if (hide) {
+        const int n = min(max(hi - k0, 0), kKeys);
+        w[0] = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+        w[1] = n >= 64 ? 0xffffffffu : n <= 32 ? 0u : (1u << (n - 32)) - 1u;
+        if (docs) {
+          const uint4 mine = document_bits(docs + k0, min(a.sk - k0, kKeys), doc);
+          w[0] &= mine.x;
+          w[1] &= mine.y;
+        }
+      }
       ok = wait_warp(&s_full[buf], (uint32_t)(t >> 1) & 1u);
       if (!ok) break;
       tc_fence_after();
@@ -337,13 +349,6 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         for (int i = 0; i < kKeys; ++i) x[i] = fmaf(-slope, fabsf(gap - (float)i), x[i]);
       }
       if (hide) {
-        const int n = min(max(hi - k0, 0), kKeys);
-        uint32_t w[2] = {n >= 32 ? 0xffffffffu : (1u << n) - 1u, n >= 64 ? 0xffffffffu : n <= 32 ? 0u : (1u << (n - 32)) - 1u};
-        if (docs) {
-          const uint4 mine = document_bits(docs + k0, min(a.sk - k0, kKeys), doc);
-          w[0] &= mine.x;
-          w[1] &= mine.y;
-        }
 #pragma unroll
         for (int i = 0; i < kKeys; ++i)
           if (!((w[i >> 5] >> (i & 31)) & 1u)) x[i] = -CUDART_INF_F;

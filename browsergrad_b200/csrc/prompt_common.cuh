@@ -19,7 +19,7 @@ constexpr int kMaxPos = 1 << 30;
 
 // Bits of the keys (of `keys` that exist from docs on) whose document is this lane's.  Each key's id is read once per warp;
 // the rows of a warp belong to few documents, so the words are made per document, by ballots, not per row.
-static __device__ __noinline__ uint4 document_bits(const int* docs, int keys, int doc) {
+__device__ __forceinline__ uint4 document_bits(const int* docs, int keys, int doc) {
   const int lane = threadIdx.x & 31;
   int id[4];
 #pragma unroll
@@ -35,22 +35,25 @@ static __device__ __noinline__ uint4 document_bits(const int* docs, int keys, in
   }
   return w;
 }
-// The sequence's length; one outside the cache is reported and cut.
-__device__ __forceinline__ int length_of(const DecoderAttention& a, int b) {
-  if (!a.lengths) return a.sk;
-  const int n = __ldg(a.lengths + b);
-  if (n >= 0 && n <= a.sk) return n;
-  if (threadIdx.x == 0) { *a.status.host = BG_ERR_INDEX_RANGE; *a.status.device = BG_ERR_INDEX_RANGE; }
-  return min(max(n, 0), a.sk);
+// What a CTA's sequence is about; the three are requested together.  A length outside the cache is reported and cut.
+struct Sequence {
+  int len, prefix;
+  long long start;
+};
+__device__ __forceinline__ Sequence sequence_of(const DecoderAttention& a, int b) {
+  const int n = a.lengths ? __ldg(a.lengths + b) : a.sk, st = a.starts ? __ldg(a.starts + b) : 0, pre = a.prefixes ? __ldg(a.prefixes + b) : 0;
+  if ((n < 0 || n > a.sk) && threadIdx.x == 0) { *a.status.host = BG_ERR_INDEX_RANGE; *a.status.device = BG_ERR_INDEX_RANGE; }
+  const int len = min(max(n, 0), a.sk);
+  return Sequence{len, pre, a.starts ? (long long)st : (long long)len - a.sq};
 }
 
 // Rows [i0, i1] of sequence b: the positions among them that see any key, and how many keys the last of them sees.
 struct Reach {
   int first, last, keys;       // first > last: none
 };
-__device__ __forceinline__ Reach reach_of(const DecoderAttention& a, int b, int len, int i0, int i1) {
-  const long long start = a.starts ? (long long)a.starts[b] : (long long)len - a.sq;
-  long long p0 = start + i0, p1 = start + i1;
+__device__ __forceinline__ Reach reach_of(const DecoderAttention& a, const Sequence& q, int i0, int i1) {
+  const int len = q.len;
+  long long p0 = q.start + i0, p1 = q.start + i1;
   if (!a.causal) {
     p0 = min(max(p0, (long long)-kMaxPos), (long long)kMaxPos);
     p1 = min(max(p1, (long long)-kMaxPos), (long long)kMaxPos);
@@ -59,29 +62,30 @@ __device__ __forceinline__ Reach reach_of(const DecoderAttention& a, int b, int 
   p0 = max(p0, 0ll);
   p1 = min(p1, (long long)len - 1);
   if (i0 > i1 || p0 > p1) return Reach{1, 0, 0};
-  return Reach{(int)p0, (int)p1, (int)min((long long)len, max(p1 + 1, (long long)(a.prefixes ? a.prefixes[b] : 0)))};
+  return Reach{(int)p0, (int)p1, (int)min((long long)len, max(p1 + 1, (long long)q.prefix))};
 }
 
 // Which tiles of KEYS keys rows [i0, i1] need: those in front of the last row's reach that, with documents, hold an id
 // between the rows' smallest and largest.
 template <int KEYS>
-__device__ __forceinline__ void needed_tiles(const DecoderAttention& a, int b, int len, int i0, int i1, unsigned char* need, int tid, int threads) {
-  const int n_kv = (len + KEYS - 1) / KEYS;
-  const int2* ranges = a.documents ? a.doc_ranges + (long long)b * ((a.sk + kDocBlock - 1) / kDocBlock) : nullptr;
-  const Reach r = reach_of(a, b, len, i0, i1);
+__device__ __forceinline__ void needed_tiles(const DecoderAttention& a, int b, const Sequence& q, int i0, int i1, unsigned char* need, int tid, int threads) {
+  const int n_kv = (q.len + KEYS - 1) / KEYS, blocks = (a.sk + kDocBlock - 1) / kDocBlock;
+  const int2* ranges = a.documents ? a.doc_ranges + (long long)b * blocks : nullptr;
+  const Reach r = reach_of(a, q, i0, i1);
   int lo = INT_MAX, hi = -1;
-  if (ranges)
-    for (int t = max(r.first, 0) / kDocBlock; r.first <= r.last && r.last >= 0 && t <= min(r.last, a.sk - 1) / kDocBlock; ++t) {
-      const int2 x = __ldg(ranges + t);
-      lo = min(lo, x.x & 0x7fffffff);
-      hi = max(hi, x.y);
-    }
+  if (ranges && r.first <= r.last && r.last >= 0) {
+    // at most 128 rows lie in two blocks
+    const int t0 = min(max(r.first, 0) / kDocBlock, blocks - 1), t1 = min(r.last / kDocBlock, blocks - 1);
+    const int2 x = __ldg(ranges + t0), y = __ldg(ranges + t1);
+    lo = min(x.x & 0x7fffffff, y.x & 0x7fffffff);
+    hi = max(x.y, y.y);
+  }
   const int end = (r.keys + KEYS - 1) / KEYS;
   for (int j = tid; j < n_kv; j += threads) {
     bool n = j < end;
-    if (n && ranges) {
+    if (ranges) {
       const int2 x = __ldg(ranges + j * KEYS / kDocBlock);
-      n = (x.x & 0x7fffffff) <= hi && x.y >= lo;
+      n = n && (x.x & 0x7fffffff) <= hi && x.y >= lo;
     }
     need[j] = n;
   }
