@@ -9,6 +9,7 @@ namespace {
 // Smallest and largest id of each 128 keys (ids below zero belong to no document, see DecoderAttention::doc_ranges).
 // One warp per block.
 __global__ void doc_ranges_kernel(const int* documents, int b, int sk, int blocks, int2* ranges) {
+  grid_launch_dependents();
   const long long w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
   if (w >= (long long)b * blocks) return;
   const int batch = (int)(w / blocks), blk = (int)(w % blocks), lane = threadIdx.x & 31;

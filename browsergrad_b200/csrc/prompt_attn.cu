@@ -2,7 +2,8 @@
 // the tensor cores of this generation.
 //
 // A CTA owns 256 consecutive query rows of one head as two tiles of 128 (A, B) that share the key and value tiles in
-// shared memory; while the softmax of one tile runs, the products of the other do.
+// shared memory; while the softmax of one tile runs, the products of the other do.  (Or one tile of 128, with two CTAs on
+// an SM: launch_prompt_attention says when.)
 //   warp 0       producer (lane 0: Q, then K tiles; lane 1: V tiles; TMA)
 //   warps 1, 2   issue the products of tile A and of tile B: S = Q K^T into tensor memory, O += P V with P read from there
 //   warp 3       clears the value rows of the tile the sequence ends in that lie behind its length: a probability of zero
@@ -39,23 +40,26 @@ using attn::ex2_approx;
 using attn::fmax3;
 using attn::tma_load_4d;
 
-constexpr int kRows = 128, kKeys = 128, kThreads = 384;
+constexpr int kRows = 128, kKeys = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyLog2 = 8.0f;
-// Registers move from warps 0-3 to the softmax warps: (128 x 72 + 256 x 216) / 384 = 168 a thread, what the CTA is
-// launched with (checked at launch; a request beyond the pool would wait for ever).
-constexpr int kLaunchRegs = 168, kLightRegs = 72, kSoftmaxRegs = 216;
-static_assert(128 * kLightRegs + 256 * kSoftmaxRegs <= kLaunchRegs * kThreads, "setmaxnreg requests exceed the CTA's registers");
-
-template <int D>
+// D: values of a head, padded; NT: query tiles of a CTA.
+template <int D, int NT>
 struct Cfg {
   static constexpr bool Alias = D == 128;                    // P in the columns of S
+  static constexpr int Threads = 128 + 128 * NT, PerSm = NT == 1 ? 2 : 1;
   static constexpr int Boxes = D / 64;                       // 128-byte wide boxes of a row
   static constexpr int BoxBytes = 128 * 128;                 // 128 rows of 64 values
   static constexpr int TileBytes = Boxes * BoxBytes;
   static constexpr int Stages = 2;
-  static constexpr int ColS = 0, ColO = 256, ColP = Alias ? 0 : 384, StepP = Alias ? 128 : 64;
-  static constexpr int Smem = 2 * TileBytes + 2 * Stages * TileBytes;
+  static constexpr int TmemCols = 256 * NT;
+  static constexpr int ColS = 0, ColO = 128 * NT, ColP = Alias ? 0 : 192 * NT, StepP = Alias ? 128 : 64;
+  static constexpr int Smem = NT * TileBytes + 2 * Stages * TileBytes;
+  // Registers move from warps 0-3 to the softmax warps, within what the CTA is launched with (checked at launch; a request
+  // beyond the pool would wait for ever).
+  static constexpr int LaunchRegs = NT == 1 ? 128 : 168, LightRegs = NT == 1 ? 56 : 72, SoftmaxRegs = NT == 1 ? 200 : 216;
+  static_assert(128 * LightRegs + 128 * NT * SoftmaxRegs <= LaunchRegs * Threads, "setmaxnreg requests exceed the CTA's registers");
+  static_assert(Alias ? NT == 2 : true, "tensor memory");
 };
 
 struct PromptParams {
@@ -98,16 +102,17 @@ __device__ __noinline__ void rescale_row(uint32_t t_o, float alpha) {
   }
 }
 
-template <bool BF16, int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool BF16, int D, int NT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(Cfg<D, NT>::Threads, Cfg<D, NT>::PerSm)
 prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const __grid_constant__ PromptParams pp) {
-  using C = Cfg<D>;
+  using C = Cfg<D, NT>;
+  constexpr int kThreads = C::Threads;
   const DecoderAttention& a = pp.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* sQ = smem;
-  unsigned char* sK = sQ + 2 * C::TileBytes;
+  unsigned char* sK = sQ + NT * C::TileBytes;
   unsigned char* sV = sK + C::Stages * C::TileBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + C::Stages * C::TileBytes);
   uint64_t* q_full = bars;                       // [2]
@@ -125,14 +130,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   unsigned char* s_need = reinterpret_cast<unsigned char*>(tmem_holder + 4);     // [2][n_kv]
 
+  if (a.documents) grid_dependency_wait();       // the ranges of their ids come from the launch before
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int n_bh = a.b * a.hq;
-  const int n_qt = (a.sq + kRows - 1) / kRows, n_pairs = (n_qt + 1) / 2;
+  const int n_qt = (a.sq + kRows - 1) / kRows, n_pairs = (n_qt + NT - 1) / NT;
   const int pair = n_pairs - 1 - (int)(blockIdx.x / (unsigned)n_bh);       // the last rows see the most keys: they go first
   const int bh = (int)(blockIdx.x % (unsigned)n_bh);
   const int b = bh / a.hq, h = bh % a.hq, hk = h / a.group;
-  const bool has_b = 2 * pair + 1 < n_qt;
+  const bool has_b = NT == 2 && 2 * pair + 1 < n_qt;
 
   const Sequence seq = sequence_of(a, b);
   const int len = seq.len;
@@ -140,8 +146,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const int2* ranges = a.documents ? a.doc_ranges + (long long)b * ((a.sk + kDocBlock - 1) / kDocBlock) : nullptr;
   const int* docs = a.documents ? a.documents + (long long)b * a.sk : nullptr;
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
-    needed_tiles<kKeys>(a, b, seq, (2 * pair + g) * kRows, min((2 * pair + g + 1) * kRows, a.sq) - 1, s_need + g * n_kv, threadIdx.x, kThreads);
+  for (int g = 0; g < NT; ++g)
+    needed_tiles<kKeys>(a, b, seq, (NT * pair + g) * kRows, min((NT * pair + g + 1) * kRows, a.sq) - 1, s_need + g * n_kv, threadIdx.x, kThreads);
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
       mbar_init(&q_full[g], 1);
@@ -149,8 +155,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       mbar_init(&p_full[g], 4); mbar_init(&pv_full[g], 1);
     }
     for (int s = 0; s < C::Stages; ++s) {
-      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 2);       // a slot is free once both issuers are done with it
-      mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 2);
+      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], NT);      // a slot is free once the issuers are done with it
+      mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], NT);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
     mbar_init(v_clean, 1);
@@ -158,25 +164,25 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "n"(C::TmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  auto next = [&](int j) { while (j < n_kv && !s_need[j] && !s_need[n_kv + j]) ++j; return j; };
+  auto next = [&](int j) { while (j < n_kv && !s_need[j] && (NT == 1 || !s_need[n_kv + j])) ++j; return j; };
   // the tile that holds both keys of the sequence and rows behind it (rows behind the buffer arrive as zeros anyway)
   const int ragged = len < a.sk && (len % kKeys) != 0 ? len / kKeys : -1;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLightRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::LightRegs));
     if (warp == 0) {
       if (lane == 0) {
         for (int g = 0; g < (has_b ? 2 : 1); ++g) {
           mbar_expect_tx(&q_full[g], C::TileBytes);
           for (int x = 0; x < C::Boxes; ++x)
-            tma_load_4d(&tmQ, sQ + g * C::TileBytes + x * C::BoxBytes, &q_full[g], x * 64, (2 * pair + g) * kRows, h, b);
+            tma_load_4d(&tmQ, sQ + g * C::TileBytes + x * C::BoxBytes, &q_full[g], x * 64, (NT * pair + g) * kRows, h, b);
         }
         int u = 0;
         for (int j = next(0); j < n_kv; j = next(j + 1), ++u) {
@@ -196,7 +202,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           for (int x = 0; x < C::Boxes; ++x) tma_load_4d(&tmV, sV + s * C::TileBytes + x * C::BoxBytes, &v_full[s], x * 64, j * kKeys, hk, b);
         }
       }
-    } else if (warp <= 2) {
+    } else if (warp <= NT) {
       const int g = warp - 1;
       const unsigned char* need = s_need + g * n_kv;
       const uint32_t q_addr = smem_u32(sQ + g * C::TileBytes);
@@ -271,7 +277,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         jc = jn;
         ++u;
       }
-    } else if (ragged >= 0) {
+    } else if (warp == 3 && ragged >= 0) {
       // warp 3: the value rows behind the sequence in its last tile
       int u = 0, j = next(0);
       for (; j < n_kv && j != ragged; j = next(j + 1)) ++u;
@@ -290,10 +296,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SoftmaxRegs));
     const int g = (warp - 4) >> 2, quarter = warp & 3;
     const int r_in_tile = quarter * 32 + lane;
-    const int row = (2 * pair + g) * kRows + r_in_tile;
+    const int row = (NT * pair + g) * kRows + r_in_tile;
     const bool active = g == 0 || has_b, row_ok = active && row < a.sq;
     if (active) {
       const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
@@ -310,14 +316,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const int pos = me.first;
       const float slope = BIAS && a.slopes ? a.slopes[h] * kLog2e : 0.f;
       const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_cap = CAP ? a.scale / a.cap : 0.f;
-      constexpr bool TURNS = C::Alias || CAP || BIAS;      // (4 x 16 heads, 4096 rows: plain scores of heads of 64 are 8 % slower with turns, the others 2 to 9 % faster)
+      constexpr bool TURNS = NT == 2 && (C::Alias || CAP || BIAS);      // (4 x 16 heads, 4096 rows: plain scores of heads of 64 are 8 % slower with turns, the others 2 to 9 % faster)
       constexpr bool FOLD = !CAP && !BIAS;        // the scale is applied in the exponent (it is positive then)
       float m_ref = -CUDART_INF_F, l = 0.f;
       bool ok = true;
       int t = 0, n_shared = 0;
       for (int j = 0; j < n_kv && ok; ++j) {
         if (!need[j]) continue;
-        const bool shared = s_need[j] && s_need[n_kv + j];
+        const bool shared = NT == 2 && s_need[j] && s_need[n_kv + j];
         const int k0 = j * kKeys;
         bool whole = hi >= k0 + kKeys;
         if (docs) {
@@ -516,35 +522,37 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   }
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(C::TmemCols) : "memory");
   }
 }
 
-template <int D>
-size_t smem_bytes(int sk) { return (size_t)Cfg<D>::Smem + 1024 + 256 + 2 * (size_t)((sk + kKeys - 1) / kKeys); }
+template <int D, int NT>
+size_t smem_bytes(int sk) { return (size_t)Cfg<D, NT>::Smem + 1024 + 256 + NT * (size_t)((sk + kKeys - 1) / kKeys); }
 
-template <bool BF16, int D, bool CAP, bool BIAS>
+template <bool BF16, int D, int NT, bool CAP, bool BIAS>
 cudaError_t launch_kernel(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
-  auto kern = prompt_attention_kernel<BF16, D, CAP, BIAS>;
+  auto kern = prompt_attention_kernel<BF16, D, NT, CAP, BIAS>;
   static const int regs = [&] {
     cudaFuncAttributes fa;
     return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
   }();
-  if (regs < kLaunchRegs) return cudaErrorLaunchOutOfResources;
-  const size_t smem = smem_bytes<D>(p.a.sk);
+  if (regs < Cfg<D, NT>::LaunchRegs) return cudaErrorLaunchOutOfResources;
+  const size_t smem = smem_bytes<D, NT>(p.a.sk);
   cudaError_t e = allow_shared(kern, smem);
   if (e != cudaSuccess) return e;
-  const int pairs = ((p.a.sq + kRows - 1) / kRows + 1) / 2;
-  kern<<<(unsigned)((long long)pairs * p.a.b * p.a.hq), kThreads, smem, s>>>(q, k, v, p);
+  const int pairs = ((p.a.sq + kRows - 1) / kRows + NT - 1) / NT;
+  const dim3 grid((unsigned)((long long)pairs * p.a.b * p.a.hq)), block(Cfg<D, NT>::Threads);
+  if (p.a.documents) return launch_dependent(kern, grid, block, smem, s, q, k, v, p);
+  kern<<<grid, block, smem, s>>>(q, k, v, p);
   return cudaGetLastError();
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, int NT>
 cudaError_t launch_rules(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
   // a scale that is not positive cannot be taken out of the row maximum: such scores are scaled like biased ones
   const bool bias = p.a.slopes || !(p.a.scale > 0.f), cap = p.a.cap > 0.f;
-  if (cap) return bias ? launch_kernel<BF16, D, true, true>(p, q, k, v, s) : launch_kernel<BF16, D, true, false>(p, q, k, v, s);
-  return bias ? launch_kernel<BF16, D, false, true>(p, q, k, v, s) : launch_kernel<BF16, D, false, false>(p, q, k, v, s);
+  if (cap) return bias ? launch_kernel<BF16, D, NT, true, true>(p, q, k, v, s) : launch_kernel<BF16, D, NT, true, false>(p, q, k, v, s);
+  return bias ? launch_kernel<BF16, D, NT, false, true>(p, q, k, v, s) : launch_kernel<BF16, D, NT, false, false>(p, q, k, v, s);
 }
 
 }  // namespace
@@ -555,8 +563,8 @@ bool prompt_attention_usable(const DecoderAttention& p, int dtype) {
   // Below 64 rows a head most of a 128-row tile would stand empty, and the key-split kernel reads each key once for the
   // whole group.
   if (p.sq < 64) return false;
-  if (smem_bytes<128>(p.sk) > 227 * 1024) return false;
-  if ((long long)((p.sq + 255) / 256) * p.b * p.hq > 0x7fffffffll) return false;
+  if (smem_bytes<128, 2>(p.sk) > 227 * 1024) return false;
+  if ((long long)((p.sq + 127) / 128) * p.b * p.hq > 0x7fffffffll) return false;
   return view_fits(p.q, dtype, p.b, p.sq, p.hq) && view_fits(p.k, dtype, p.b, p.sk, p.hkv) && view_fits(p.v, dtype, p.b, p.sk, p.hkv) && view_fits(p.out, dtype, p.b, p.sq, p.hq);
 }
 
@@ -571,8 +579,13 @@ cudaError_t launch_prompt_attention(const DecoderAttention& p, int dtype, cudaSt
   pp.a = p;
   pp.idesc_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
   pp.idesc_pv = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)((wide ? 128 : 64) >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);   // V is MN-major
-  if (wide) return bf ? launch_rules<true, 128>(pp, q, k, v, s) : launch_rules<false, 128>(pp, q, k, v, s);
-  return bf ? launch_rules<true, 64>(pp, q, k, v, s) : launch_rules<false, 64>(pp, q, k, v, s);
+  if (wide) return bf ? launch_rules<true, 128, 2>(pp, q, k, v, s) : launch_rules<false, 128, 2>(pp, q, k, v, s);
+  // One query tile a CTA and two CTAs an SM where there is little work behind a CTA's start, which the other then covers:
+  // 32 x 128 tokens 18 us against 24, 16 x 512 33 against 35 (capped 45 against 49), packed documents of 400 in 4 x 2048
+  // 46 against 49; from 2048 keys on two tiles that share their keys and take turns win (capped 99.5 us against 101.5,
+  // 16 heads of 4096 keys 683 against 773).
+  if (p.documents || p.sk <= 1024) return bf ? launch_rules<true, 64, 1>(pp, q, k, v, s) : launch_rules<false, 64, 1>(pp, q, k, v, s);
+  return bf ? launch_rules<true, 64, 2>(pp, q, k, v, s) : launch_rules<false, 64, 2>(pp, q, k, v, s);
 }
 
 }  // namespace bg

@@ -121,6 +121,7 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   unsigned char* s_need = reinterpret_cast<unsigned char*>(tmem_holder + 4);     // [n_kv]
 
+  if (a.documents) grid_dependency_wait();       // the ranges of their ids come from the launch before
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int n_bh = a.b * a.hq;
@@ -462,7 +463,9 @@ cudaError_t launch_kernel(const Prompt32Params& p, const CUtensorMap& q, const C
   const size_t smem = smem_bytes(p.a.sk);
   cudaError_t e = allow_shared(kern, smem);
   if (e != cudaSuccess) return e;
-  kern<<<(unsigned)((long long)((p.a.sq + kRows - 1) / kRows) * p.a.b * p.a.hq), kThreads, smem, s>>>(q, k, v, p);
+  const dim3 grid((unsigned)((long long)((p.a.sq + kRows - 1) / kRows) * p.a.b * p.a.hq));
+  if (p.a.documents) return launch_dependent(kern, grid, dim3(kThreads), smem, s, q, k, v, p);
+  kern<<<grid, kThreads, smem, s>>>(q, k, v, p);
   return cudaGetLastError();
 }
 
