@@ -31,7 +31,7 @@ typedef unsigned long long u64;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBuckets = 2048, kCoarse = 64;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxListed = 1024;     // keys of one bucket that are sorted
+constexpr int kMaxListed = kThreads; // keys of one bucket that are sorted, one a thread
 constexpr int kMaxPairs = 256;       // keys that are ranked by comparing all pairs
 
 __device__ __forceinline__ float widen(float v) { return v; }
@@ -151,17 +151,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     return e >= 0 && e < p.vocab ? key_of(widen(x[e])) : 0u;
   };
 
-  // f(key, place in the slice) for [j0, j1), four at a time by `lanes` threads of which this is number `me`; j0 a multiple of four
-  auto each_key = [&](int j0, int j1, int me, int lanes, auto&& f) {
-#pragma unroll 2
+  // f(four keys, place of the first in the slice) for [j0, j1) by `lanes` threads of which this is number `me`; j0 a multiple of four
+  auto each_four = [&](int j0, int j1, int me, int lanes, auto&& f) {
     for (int j = j0 + 4 * me; j < j1; j += 4 * lanes) {
-      uint4 k;
-      if (RES) k = *reinterpret_cast<const uint4*>(keys + j);
-      else k = make_uint4(key_at(j), key_at(j + 1), key_at(j + 2), key_at(j + 3));
-      f(k.x, j);
-      f(k.y, j + 1);
-      f(k.z, j + 2);
-      f(k.w, j + 3);
+      uint32_t k[4];
+      if (RES) *reinterpret_cast<uint4*>(k) = *reinterpret_cast<const uint4*>(keys + j);
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = key_at(j + i);
+      f(k, j);
     }
   };
 
@@ -258,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
 
   int round = 0;
-  // One round: `add(key)` for this CTA's keys and `once()` for the cluster, then the bucket
+  // One round: `add(four keys)` for this CTA's keys and `once()` for the cluster, then the bucket
   // in which the running sum (bucket 0 first) reaches the target.  target_of(total) gives the target from the round's
   // total.
   auto search = [&](auto&& add, auto&& once, auto&& target_of) {
@@ -269,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     ++round;
     if (rank == 0 && tid == 0) once();
-    each_key(0, slice, tid, kThreads, [&](uint32_t k, int) { add(k); });
+    each_four(0, slice, tid, kThreads, [&](const uint32_t* k, int) { add(k); });
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kCoarse / kWarps; ++i) {
@@ -316,11 +314,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // Collects the cluster's keys that `wanted` names into all_listed and returns their number; the list holds them when
   // there are at most kMaxListed.  `n_listed` is zero before; the lists may be read until the next cluster barrier.
   auto collect = [&](auto&& wanted) -> uint32_t {
-    each_key(0, slice, tid, kThreads, [&](uint32_t k, int j) {
-      if (k && wanted(k)) {
-        const uint32_t at = atomicAdd(&sh.n_listed, 1u);
-        if (at < kMaxListed) sh.listed[at] = (u64)k << 32 | (uint32_t)~(uint32_t)(begin + j);
-      }
+    each_four(0, slice, tid, kThreads, [&](const uint32_t* k, int j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k[i] && wanted(k[i])) {
+          const uint32_t at = atomicAdd(&sh.n_listed, 1u);
+          if (at < kMaxListed) sh.listed[at] = (u64)k[i] << 32 | (uint32_t)~(uint32_t)(begin + j + i);
+        }
     });
     cluster.sync();
     u64* all = sh.all_listed();
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     for (int r = 0; r < kMaxCluster; ++r) m[r] = r < nc ? cluster.map_shared_rank(&sh, r)->n_listed : 0u;
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) {
-      for (uint32_t i = tid; i < m[r] && n + i < kMaxListed; i += kThreads) all[n + i] = cluster.map_shared_rank(&sh, r)->listed[i];
+      if (tid < m[r] && n + tid < kMaxListed) all[n + tid] = cluster.map_shared_rank(&sh, r)->listed[tid];
       n += m[r];
     }
     __syncthreads();
@@ -364,39 +364,36 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       }
     }
     if (held <= kMaxListed) {
-      const int n = (int)held;
+      // Bitonic, largest first, an element a thread: by shuffles inside a warp, through shared memory across warps.
+      const int n = (int)held, log = n <= 1 ? 0 : 32 - __clz(n - 1);
       u64* all = sh.all_listed();
-      const int log = n <= 1 ? 0 : 32 - __clz(n - 1), padded = 1 << log;
-      for (int i = n + tid; i < padded; i += kThreads) all[i] = 0ull;
+      u64 e = tid < n ? all[tid] : 0ull;
       __syncthreads();
-      // Bitonic, largest first; a thread takes pairs tid and tid + 512.  A warp's pairs less than 64 apart are its own.
       for (int ls = 1; ls <= log; ++ls)
         for (int ld = ls - 1; ld >= 0; --ld) {
-          for (int i = tid; i < padded / 2; i += kThreads) {
-            const int x = ((i >> ld) << (ld + 1)) | (i & ((1 << ld) - 1)), y = x + (1 << ld);
-            const u64 p0 = all[x], p1 = all[y];
-            if ((p0 < p1) == (((x >> ls) & 1) == 0)) { all[x] = p1; all[y] = p0; }
-          }
-          if (ld > 5 || (ld == 0 && ls > 5)) __syncthreads();
-          else __syncwarp();
+          u64 o;
+          if (ld >= 5) {
+            all[tid] = e;
+            __syncthreads();
+            o = all[tid ^ (1 << ld)];
+            __syncthreads();
+          } else if (warp * 32 < 1 << log) o = __shfl_xor_sync(0xffffffffu, e, 1 << ld);
+          else continue;
+          const bool first = !(tid >> ld & 1), down = !(tid >> ls & 1);
+          e = (e > o) == (first == down) ? e : o;
         }
-      __syncthreads();
-      // running sums of two neighbours a thread; the one that reaches what is wanted is the cut
-      const int i0 = 2 * tid;
-      const u64 e0 = i0 < n ? all[i0] : 0ull, e1 = i0 + 1 < n ? all[i0 + 1] : 0ull;
-      const u64 f0 = !e0 ? 0ull : counting ? 1ull : w.fixed_of((uint32_t)(e0 >> 32)), f1 = !e1 ? 0ull : counting ? 1ull : w.fixed_of((uint32_t)(e1 >> 32));
-      const u64 in_warp = warp_scan(f0 + f1, lane);
+      all[tid] = e;
+      // running sums; the element that reaches what is wanted is the cut
+      const u64 f = !e ? 0ull : counting ? 1ull : w.fixed_of((uint32_t)(e >> 32));
+      const u64 in_warp = warp_scan(f, lane);
       if (lane == 31) sh.warp_sum[warp] = in_warp;
       __syncthreads();
-      u64 before = in_warp - f0 - f1;
+      u64 before = in_warp - f;
       for (int i = 0; i < warp; ++i) before += sh.warp_sum[i];
-      int at = -1;
-      if (before < wanted && before + f0 >= wanted) at = i0;
-      else if (before + f0 < wanted && before + f0 + f1 >= wanted) at = i0 + 1;
-      if (at >= 0) {                       // exactly one thread
-        const uint32_t key = (uint32_t)(all[at] >> 32);
+      if (before < wanted && before + f >= wanted) {       // exactly one thread
+        const uint32_t key = (uint32_t)(e >> 32);
         uint32_t same = 1;
-        while ((int)same <= at && (uint32_t)(all[at - (int)same] >> 32) == key) ++same;
+        while ((int)same <= tid && (uint32_t)(all[tid - (int)same] >> 32) == key) ++same;
         sh.cut_key = key;
         sh.cut_ties = same;
       }
@@ -426,10 +423,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       const int shift = max(0, 21 - __clz(hi - lo));     // 2048 buckets over the range
       auto bucket_of = [&](uint32_t k) { return (hi - k) >> shift; };
       const u64 want = wanted;
-      search([&](uint32_t k) {
-               if (k < lo || k > hi || k <= cut.key) return;
-               if (counting) atomicAdd(&sh.low[bucket_of(k)], 1u);
-               else if (const u64 f = w.fixed_of(k)) sh.add(bucket_of(k), f);
+      search([&](const uint32_t* four) {
+#pragma unroll
+               for (int i = 0; i < 4; ++i) {
+                 const uint32_t k = four[i];
+                 if (k < lo || k > hi || k <= cut.key) continue;
+                 if (counting) atomicAdd(&sh.low[bucket_of(k)], 1u);
+                 else if (const u64 f = w.fixed_of(k)) sh.add(bucket_of(k), f);
+               }
              },
              [&] {
                if (!counting && cut.ties && cut.key >= lo && cut.key <= hi) sh.add(bucket_of(cut.key), w.fixed_of(cut.key) * cut.ties);
@@ -455,7 +456,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const int top_k = p.top_ks ? p.top_ks[row] : p.top_k;
   if (top_k > 0 && top_k < p.vocab) {
     const float sc = linear_of(value_of(low));
-    search([&](uint32_t k) { if (k) atomicAdd(&sh.low[linear(k, sc)], 1u); }, [] {}, [&](u64) { return (u64)top_k; });
+    search([&](const uint32_t* k) {
+#pragma unroll
+             for (int i = 0; i < 4; ++i)
+               if (k[i]) atomicAdd(&sh.low[linear(k[i], sc)], 1u);
+           },
+           [] {}, [&](u64) { return (u64)top_k; });
     if (sh.above + sh.in_bucket <= kMaxPairs) {
       // few enough to finish on a list: ranks, the nucleus, and the draw in index order, by comparing all pairs
       const uint32_t b0 = sh.bucket;
@@ -508,9 +514,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (top_p < 1.0f) {
     const float sc = linear_of(fmaxf(value_of(low), w.top_value - 34.0f * t));
     const Cut by_rank = cut;
-    search([&](uint32_t k) {
-             const u64 f = w.fixed_of(k);
-             if (k > by_rank.key && f) sh.add(linear(k, sc), f);
+    search([&](const uint32_t* k) {
+             u64 f[4];                     // all four ahead of the first atomic, which the table's loads cannot pass
+#pragma unroll
+             for (int i = 0; i < 4; ++i) f[i] = w.fixed_of(k[i]);
+#pragma unroll
+             for (int i = 0; i < 4; ++i)
+               if (k[i] > by_rank.key && f[i]) sh.add(linear(k[i], sc), f[i]);
            },
            [&] { if (by_rank.ties) sh.add(linear(by_rank.key, sc), w.fixed_of(by_rank.key) * by_rank.ties); },
            nucleus);
@@ -524,10 +534,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   {
     u64 sum = 0;
     uint32_t ties = 0;
-    each_key(s0, s1, lane, 32, [&](uint32_t k, int) {
-      const u64 f = w.drawn(k);
-      sum += k > cut.key ? f : 0ull;
-      ties += k == cut.key;
+    each_four(s0, s1, lane, 32, [&](const uint32_t* k, int) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u64 f = w.drawn(k[i]);
+        sum += k[i] > cut.key ? f : 0ull;
+        ties += k[i] == cut.key;
+      }
     });
     if (cut.key == 0u) ties = 0u;
     sum = warp_sum(sum);
