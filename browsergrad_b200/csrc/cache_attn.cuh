@@ -290,6 +290,10 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
 #pragma unroll
     for (int n = 0; n < KT / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
     if constexpr (C::ES == 2) {
+      // a chain of dependent products is as long as the head: odd steps go to one of their own
+      float s2[KT / 8][4];
+#pragma unroll
+      for (int n = 0; n < KT / 8; ++n) s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
         uint32_t a[4];
@@ -301,14 +305,25 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
         for (int n = 0; n < KT / 16; ++n) {
           uint32_t kf[4];
           ldsm4(kf, tk + (n * 16 + (lane >> 4) * 8 + (lane & 7)) * LD + kk * 16 + ((lane >> 3) & 1) * 8);
-          mma16<T>(s[2 * n], a, kf[0], kf[1]);
-          mma16<T>(s[2 * n + 1], a, kf[2], kf[3]);
+          mma16<T>(kk & 1 ? s2[2 * n] : s[2 * n], a, kf[0], kf[1]);
+          mma16<T>(kk & 1 ? s2[2 * n + 1] : s[2 * n + 1], a, kf[2], kf[3]);
         }
       }
+#pragma unroll
+      for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
     } else {
       const float* qf = reinterpret_cast<const float*>(sQ) + ra * LD + t4;
       const float* kf = reinterpret_cast<const float*>(tk) + g * LD + t4;
-#pragma unroll 4
+      // Four chains for hi.hi and one for the small products: the tensor core truncates as it adds, a bias of half a step
+      // each time, which a single chain of the whole head would raise to 10^-6 of the score; and they run side by side.
+      float c[KT / 8][5][4];
+#pragma unroll
+      for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 5; ++j) c[n][j][0] = c[n][j][1] = c[n][j][2] = c[n][j][3] = 0.f;
+#pragma unroll
       for (int kk = 0; kk < DP / 8; ++kk) {
         uint32_t ah[4], al[4];
         split_tf32(qf[kk * 8], ah[0], al[0]);
@@ -320,11 +335,15 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
           uint32_t bh2[2], bl2[2];
           split_tf32(kf[n * 8 * LD + kk * 8], bh2[0], bl2[0]);
           split_tf32(kf[n * 8 * LD + kk * 8 + 4], bh2[1], bl2[1]);
-          mma_tf32(s[n], al, bh2);
-          mma_tf32(s[n], ah, bl2);
-          mma_tf32(s[n], ah, bh2);
+          mma_tf32(c[n][4], al, bh2);
+          mma_tf32(c[n][kk & 3], ah, bh2);
+          mma_tf32(c[n][4], ah, bl2);
         }
       }
+#pragma unroll
+      for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = ((c[n][0][e] + c[n][1][e]) + (c[n][2][e] + c[n][3][e])) + c[n][4][e];
     }
     // scores -> the exponent's unit (powers of two), rules, maximum
     float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
