@@ -490,6 +490,225 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
   }
 }
 
+// fp32 with at most four query rows a key head: no tensor core.  Sixteen MMA rows would stand empty, and splitting every
+// key and value into tf32 parts costs more instructions than the products (8 heads of 53307 keys of 128: 121 us that way).
+// A warp owns tiles of eight keys.  Scores: four lanes a key, each a quarter of the head, for every row; then each of the
+// four has one row's score.  P V: a lane holds four values of the result of every row and takes the probabilities by
+// shuffle.  All in plain 32-bit arithmetic; groups and splits are joined as above.
+template <int DP_, int R_>
+struct FewCfg {
+  static constexpr int DP = DP_, R = R_, KT = 8, Warps = DP > 128 ? 4 : 8, Threads = Warps * 32;
+  static constexpr int LD = DP % 32 == 0 ? DP + 16 : DP;         // rows of two keys lie 16 banks apart
+  static constexpr int TileFloats = KT * LD;
+  static constexpr int Stages = 2;
+  static constexpr int RingBytes = Stages * Warps * 2 * TileFloats * 4;
+  static constexpr int QBytes = R * DP * 4;
+  static constexpr int MergeBytes = Warps * R * DP * 4;
+  static constexpr int Smem = QBytes + (RingBytes > MergeBytes ? RingBytes : MergeBytes);
+};
+
+template <int DP, int R>
+__global__ void __launch_bounds__(FewCfg<DP, R>::Threads, DP <= 64 ? 2 : 1)
+few_rows_kernel(const __grid_constant__ DecoderAttention p, int splits, int vec, float* partials) {
+  using C = FewCfg<DP, R>;
+  constexpr int KT = C::KT, LD = C::LD, KG = C::Warps, ST = C::Stages, ROWS = 16;      // (partial results keep the layout of 16 rows)
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* sQ = reinterpret_cast<float*>(smem);
+  float* ring = reinterpret_cast<float*>(smem + C::QBytes);
+  __shared__ int s_hi[4], s_pos[4], s_doc[4];
+  __shared__ float s_m[C::Warps * 4], s_l[C::Warps * 4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int unit = blockIdx.x / splits, split = blockIdx.x % splits;
+  const int b = unit / p.hkv, hk = unit % p.hkv, n_rows = p.group * p.sq;
+  const int len_in = p.lengths ? __ldg(p.lengths + b) : p.sk, start_in = p.starts ? __ldg(p.starts + b) : 0, prefix = p.prefixes ? __ldg(p.prefixes + b) : 0;
+  const int len = min(max(len_in, 0), p.sk);
+  if (len != len_in && tid == 0) { *p.status.host = BG_ERR_INDEX_RANGE; *p.status.device = BG_ERR_INDEX_RANGE; }
+  if (tid < 4) {
+    int hi = 0, doc = -1;
+    long long pos = 0;
+    if (tid < n_rows) {
+      pos = (p.starts ? (long long)start_in : (long long)len - p.sq) + tid / p.group;
+      if (!p.causal) hi = len;
+      else if (pos >= 0 && pos < len) hi = min((long long)len, max(pos + 1, (long long)prefix));
+      if (p.documents) {
+        doc = pos >= 0 && pos < p.sk ? p.documents[(long long)b * p.sk + pos] : -1;
+        if (doc < 0) hi = 0;
+      }
+    }
+    s_hi[tid] = hi;
+    s_pos[tid] = (int)min(max(pos, (long long)-kMaxPos), (long long)kMaxPos);
+    s_doc[tid] = doc;
+  }
+  for (int i = tid; i < R * DP; i += C::Threads) {
+    const int r = i / DP, d = i - r * DP, tok = r / p.group, gh = r - tok * p.group;
+    sQ[i] = r < n_rows && d < p.d ? reinterpret_cast<const float*>(p.q.ptr)[b * p.q.sb + tok * p.q.sr + (long long)(hk * p.group + gh) * p.q.sh + d] : 0.f;
+  }
+  __syncthreads();
+  int top = 0, doc_min = INT_MAX, doc_max = -1;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (s_hi[r] > 0) { top = max(top, s_hi[r]); doc_min = min(doc_min, s_doc[r]); doc_max = max(doc_max, s_doc[r]); }
+  const int n_tiles = (top + KT - 1) / KT;
+  const int per = ((n_tiles + splits * KG - 1) / (splits * KG)) * KG;
+  const int t_begin = split * per, t_end = min(n_tiles, t_begin + per);
+  const int2* ranges = p.documents ? p.doc_ranges + (long long)b * ((p.sk + kDocBlock - 1) / kDocBlock) : nullptr;
+  auto next = [&](int t) {
+    if (ranges)
+      while (t < t_end) {
+        const int2 rg = __ldg(ranges + t * KT / kDocBlock);
+        if ((rg.x & 0x7fffffff) <= doc_max && rg.y >= doc_min) break;
+        t += KG;
+      }
+    return t;
+  };
+  const float* kp = reinterpret_cast<const float*>(p.k.ptr) + b * p.k.sb + hk * p.k.sh;
+  const float* vp = reinterpret_cast<const float*>(p.v.ptr) + b * p.v.sb + hk * p.v.sh;
+  auto tile_ptr = [&](int stage, int which) { return ring + ((stage * KG + warp) * 2 + which) * C::TileFloats; };
+  auto load = [&](int tile, int stage) {
+    const int key0 = tile * KT;
+    float* dk = tile_ptr(stage, 0);
+    float* dv = tile_ptr(stage, 1);
+    if (vec) {
+      constexpr int CPR = DP / 4;
+#pragma unroll
+      for (int i = lane; i < KT * CPR; i += 32) {
+        const int r = i / CPR, c = (i - r * CPR) * 4;
+        const bool there = key0 + r < len && c < p.d;
+        const long long key = there ? key0 + r : 0;
+        const int col = there ? c : 0;
+        cp_async16(dk + r * LD + c, kp + key * p.k.sr + col, there);
+        cp_async16(dv + r * LD + c, vp + key * p.v.sr + col, there);
+      }
+    } else {
+      for (int i = lane; i < KT * DP; i += 32) {
+        const int r = i / DP, c = i - r * DP;
+        const bool there = key0 + r < len && c < p.d;
+        dk[r * LD + c] = there ? kp[(long long)(key0 + r) * p.k.sr + c] : 0.f;
+        dv[r * LD + c] = there ? vp[(long long)(key0 + r) * p.v.sr + c] : 0.f;
+      }
+    }
+  };
+  const int part = lane & 3, my_row = part < R ? part : part % R;
+  const int hi = s_hi[my_row], pos = s_pos[my_row], doc = s_doc[my_row];
+  const float slope = p.slopes && my_row < n_rows ? p.slopes[hk * p.group + my_row % p.group] * kLog2e : 0.f;
+  const float to_log2 = p.cap > 0.f ? p.cap * kLog2e : p.scale * kLog2e, to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f;
+  constexpr int PER = (DP + 127) / 128;
+  float4 o[R][PER];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -CUDART_INF_F, l = 0.f;                     // of my_row, the same in the eight lanes that share it
+  int lt = next(t_begin + warp), ct = lt, issued = 0, done = 0;
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) {
+    if (lt < t_end) { load(lt, issued % ST); lt = next(lt + KG); }
+    ++issued;
+    cp_async_commit();
+  }
+  while (ct < t_end) {
+    cp_async_wait<ST - 2>();
+    __syncwarp();
+    if (lt < t_end) { load(lt, issued % ST); lt = next(lt + KG); }
+    ++issued;
+    cp_async_commit();
+    const float* tk = tile_ptr(done % ST, 0) + (lane >> 2) * LD + part * 4;
+    const float* tv = tile_ptr(done % ST, 1) + lane * 4;
+    const int key = ct * KT + (lane >> 2);
+    ++done;
+    ct = next(ct + KG);
+    float acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const float4 kv = *reinterpret_cast<const float4*>(tk + i * 16);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float4 qv = *reinterpret_cast<const float4*>(sQ + r * DP + i * 16 + part * 4);
+        acc[r] = fmaf(kv.x, qv.x, fmaf(kv.y, qv.y, fmaf(kv.z, qv.z, fmaf(kv.w, qv.w, acc[r]))));
+      }
+    }
+    float y = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 1);
+      acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 2);
+      if (r == my_row) y = acc[r];
+    }
+    y = p.cap > 0.f ? to_log2 * tanhf(y * to_cap) : y * to_log2;
+    if (p.slopes) y = fmaf(-slope, fabsf((float)(pos - key)), y);
+    bool seen = key < hi;
+    if (p.documents) seen = seen && __ldg(p.documents + (long long)b * p.sk + min(key, p.sk - 1)) == doc;
+    y = seen ? y : -CUDART_INF_F;
+    float mx = y;
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float m_new = fmaxf(m, mx), m_use = m_new == -CUDART_INF_F ? 0.f : m_new;
+    const float alpha = ex2(m - m_use), pr = ex2(y - m_use);
+    m = m_new;
+    float sum = pr;
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    l = fmaf(l, alpha, sum);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float al = __shfl_sync(0xffffffffu, alpha, r);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) { o[r][i].x *= al; o[r][i].y *= al; o[r][i].z *= al; o[r][i].w *= al; }
+    }
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+      float pk[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) pk[r] = __shfl_sync(0xffffffffu, pr, k * 4 + r);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (DP % 128 != 0 && i * 128 + lane * 4 >= DP) continue;
+        const float4 v = *reinterpret_cast<const float4*>(tv + k * LD + i * 128);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          o[r][i].x = fmaf(pk[r], v.x, o[r][i].x); o[r][i].y = fmaf(pk[r], v.y, o[r][i].y);
+          o[r][i].z = fmaf(pk[r], v.z, o[r][i].z); o[r][i].w = fmaf(pk[r], v.w, o[r][i].w);
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+  grid_launch_dependents();
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (i * 128 + lane * 4 < DP) *reinterpret_cast<float4*>(ring + (warp * R + r) * DP + i * 128 + lane * 4) = o[r][i];
+  if (lane < R) { s_m[warp * 4 + lane] = m; s_l[warp * 4 + lane] = l; }
+  __syncthreads();
+  float* part_out = partials ? partials + ((long long)unit * splits + split) * (ROWS * (DP + 2)) : nullptr;
+  const int live = min(R, n_rows);
+  for (int i = tid; i < live * DP; i += C::Threads) {
+    const int r = i / DP, d = i - r * DP;
+    float top_m = -CUDART_INF_F, sum = 0.f, v = 0.f;
+#pragma unroll
+    for (int k = 0; k < KG; ++k) top_m = fmaxf(top_m, s_m[k * 4 + r]);
+    if (top_m != -CUDART_INF_F)
+#pragma unroll
+      for (int k = 0; k < KG; ++k) {
+        const float f = ex2(s_m[k * 4 + r] - top_m);
+        sum = fmaf(f, s_l[k * 4 + r], sum);
+        v = fmaf(f, ring[(k * R + r) * DP + d], v);
+      }
+    if (!part_out) {
+      const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+      const int tok = r / p.group, gh = r - tok * p.group;
+      if (d < p.d) reinterpret_cast<float*>(const_cast<void*>(p.out.ptr))[b * p.out.sb + tok * p.out.sr + (long long)(hk * p.group + gh) * p.out.sh + d] = v * inv;
+    } else {
+      part_out[r * DP + d] = v;
+      if (d == 0) { part_out[ROWS * DP + r] = top_m; part_out[ROWS * DP + ROWS + r] = sum; }
+    }
+  }
+}
+
 // Joins the parts of one row: four warps take the splits in turn, 16 bytes a lane.
 template <typename T, int DP, int RT>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ DecoderAttention p, int splits, int row_tiles, const float* partials) {
@@ -555,8 +774,30 @@ cudaError_t launch_one(const DecoderAttention& p, const CacheAttnPlan& plan, flo
   return launch_dependent(join_kernel<T, DP, RT>, dim3((unsigned)(grid / plan.splits * 16 * RT)), dim3(128), 0, s, p, plan.splits, row_tiles, (const float*)partials);
 }
 
+template <int DP, int R>
+cudaError_t launch_few(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s) {
+  using C = FewCfg<DP, R>;
+  static_assert(C::Smem + 1024 <= 227 * 1024, "shared memory of a CTA");
+  const long long grid = (long long)p.b * p.hkv * plan.splits;
+  if (grid <= 0 || grid > 0x7fffffffll) return cudaErrorInvalidValue;
+  const int vec = p.d % 4 == 0 && (reinterpret_cast<uintptr_t>(p.k.ptr) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.v.ptr) & 15) == 0 &&
+                  p.k.sr % 4 == 0 && p.v.sr % 4 == 0 && p.k.sb % 4 == 0 && p.v.sb % 4 == 0 && p.k.sh % 4 == 0 && p.v.sh % 4 == 0;
+  cudaError_t e = allow_shared(few_rows_kernel<DP, R>, C::Smem);
+  if (e != cudaSuccess) return e;
+  few_rows_kernel<DP, R><<<(unsigned)grid, C::Threads, C::Smem, s>>>(p, plan.splits, vec, plan.splits > 1 ? partials : nullptr);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || plan.splits == 1) return e;
+  return launch_dependent(join_kernel<float, DP, 1>, dim3((unsigned)(grid / plan.splits * 16)), dim3(128), 0, s, p, plan.splits, 1, (const float*)partials);
+}
+
 template <typename T, int DP>
 cudaError_t launch_rows(const DecoderAttention& p, const CacheAttnPlan& plan, float* partials, cudaStream_t s) {
+  if constexpr (sizeof(T) == 4) {
+    const int rows = p.group * p.sq;
+    if (rows == 1) return launch_few<DP, 1>(p, plan, partials, s);
+    if (rows == 2) return launch_few<DP, 2>(p, plan, partials, s);
+    if (rows <= 4) return launch_few<DP, 4>(p, plan, partials, s);
+  }
   return plan.row_tiles == 1 ? launch_one<T, DP, 1>(p, plan, partials, s)
          : plan.row_tiles == 2 ? launch_one<T, DP, 2>(p, plan, partials, s) : launch_one<T, DP, 4>(p, plan, partials, s);
 }
