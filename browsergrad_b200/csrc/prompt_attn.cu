@@ -6,8 +6,8 @@
 // an SM: launch_prompt_attention says when.)
 //   warp 0       producer (lane 0: Q, then K tiles; lane 1: V tiles; TMA)
 //   warps 1, 2   issue the products of tile A and of tile B: S = Q K^T into tensor memory, O += P V with P read from there
-//   warp 3       clears the value rows of the tile the sequence ends in that lie behind its length: a probability of zero
-//                times what an unwritten cache holds would not be zero
+//   warp 3       clears the value rows of the tile the sequence ends in that lie behind its length, between the tile's landing
+//                and its products: a probability of zero times what an unwritten cache holds would not be zero
 //   warps 4-7    softmax of tile A, one thread per query row; warps 8-11: of tile B
 // With 64 values a head P has columns of its own in tensor memory, and the scores of the next key tile are computed
 // while a tile's softmax still runs; with 128 values the 512 columns are S and O of both tiles, P takes the place of the
@@ -125,8 +125,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   uint64_t* p_full = s_empty + 2;                // [2] P is there
   uint64_t* pv_full = p_full + 2;                // [2] P V has completed
   uint64_t* turn = pv_full + 2;                  // [2][4] a warp of tile A (0) / B (1) has its exponentials of a shared key tile behind it
-  uint64_t* v_clean = turn + 8;                  // the value tile the sequence ends in has been cleared behind it
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(v_clean + 1);
+  uint64_t* v_raw = turn + 8;                    // the value tile the sequence ends in has landed, still to be cleared behind it
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(v_raw + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   unsigned char* s_need = reinterpret_cast<unsigned char*>(tmem_holder + 4);     // [2][n_kv]
 
@@ -159,7 +159,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], NT);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
-    mbar_init(v_clean, 1);
+    mbar_init(v_raw, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -198,8 +198,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         for (int j = next(0); j < n_kv; j = next(j + 1), ++u) {
           const int s = u % C::Stages;
           if (!mbar_wait(&v_empty[s], ((uint32_t)(u / C::Stages) & 1u) ^ 1u, abort_flag)) break;
-          mbar_expect_tx(&v_full[s], C::TileBytes);
-          for (int x = 0; x < C::Boxes; ++x) tma_load_4d(&tmV, sV + s * C::TileBytes + x * C::BoxBytes, &v_full[s], x * 64, j * kKeys, hk, b);
+          uint64_t* landed = j == ragged ? v_raw : &v_full[s];       // warp 3 passes the cleared tile on
+          mbar_expect_tx(landed, C::TileBytes);
+          for (int x = 0; x < C::Boxes; ++x) tma_load_4d(&tmV, sV + s * C::TileBytes + x * C::BoxBytes, landed, x * 64, j * kKeys, hk, b);
         }
       }
     } else if (warp <= NT) {
@@ -230,9 +231,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         __syncwarp();
         return true;
       };
-      auto issue_pv = [&](int slot, bool dirty) -> bool {
+      auto issue_pv = [&](int slot) -> bool {
         const int n = n_pv++;
-        if (dirty && !wait_all(v_clean, 0)) return false;
         if (!wait_all(&p_full[g], (uint32_t)n & 1u)) return false;
         tc_fence_after();
         const uint32_t v_addr = smem_u32(sV + slot * C::TileBytes);
@@ -271,7 +271,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         const int slot = u % C::Stages;
         if (ok) ok = wait_all(&v_full[slot], (uint32_t)(u / C::Stages) & 1u);
         const bool used = need[jc] != 0;
-        if (ok && used) ok = issue_pv(slot, jc == ragged);
+        if (ok && used) ok = issue_pv(slot);
         if (ok) release(&v_empty[slot], used);
         if (C::Alias && ok && jn < n_kv) scores(jn, u + 1);
         jc = jn;
@@ -283,7 +283,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       for (; j < n_kv && j != ragged; j = next(j + 1)) ++u;
       if (j == ragged) {
         const int slot = u % C::Stages;
-        if (mbar_wait(&v_full[slot], (uint32_t)(u / C::Stages) & 1u, abort_flag)) {
+        if (mbar_wait(v_raw, 0, abort_flag)) {
           const int r0 = len - ragged * kKeys;
           for (int i = lane; i < (kKeys - r0) * 8 * C::Boxes; i += 32) {      // a row is 128 bytes of each box, wherever its pieces lie
             const int x = i / ((kKeys - r0) * 8), c = i - x * ((kKeys - r0) * 8);
@@ -291,7 +291,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           }
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(v_clean);
+          if (lane == 0) mbar_arrive(&v_full[slot]);
         }
       }
     }

@@ -304,8 +304,9 @@ int decoder_attention(const Call& c, const bg_head_view* q, const bg_head_view* 
   if (hq % hkv) return c.error(BG_ERR_INVALID, "query heads must be a multiple of the key heads");
   if (hq * sq > kMaxExtent) return c.error(BG_ERR_INVALID, "too many query rows");
   if (d > 256) return c.error(BG_ERR_UNSUPPORTED, "head dimensions above 256");
-  if (!std::isfinite(rules->scale)) return c.error(BG_ERR_INVALID, "scale must be finite");
-  if (!(rules->softcap >= 0.0) || !std::isfinite(rules->softcap)) return c.error(BG_ERR_INVALID, "softcap must be zero (none) or positive");
+  // (within these the kernels' factors, scale log2 e, cap log2 e and scale / cap, are all numbers of 32 bits)
+  if (!(fabs(rules->scale) <= 1e18)) return c.error(BG_ERR_INVALID, "scale must be a number of at most 1e18");
+  if (rules->softcap != 0.0 && !(rules->softcap >= 1e-6 && rules->softcap <= 1e6)) return c.error(BG_ERR_INVALID, "softcap must be zero (none) or lie between 1e-6 and 1e6");
   if (rules->prefixes && !rules->causal) return c.error(BG_ERR_INVALID, "prefixes need causal attention");
   DecoderAttention p{};
   if (int rc = view_of(c, q, b, sq, hq, d, dtype, "q", false, &p.q)) return rc;

@@ -255,7 +255,7 @@ int bg_rotary_append(bg_context* ctx, const bg_head_view* q, const bg_head_view*
                      const bg_head_view* out_view, bg_handle* out);
 
 /* Attention of sq query rows over sk key rows, hq query heads in groups that share hkv key heads, d <= 256.
- * Row i of sequence b stands at position t = starts[b] + i (lengths[b] - sq + i when starts is 0: the rows are the last
+ * |scale| <= 1e18; softcap is 0 (none) or in [1e-6, 1e6].  Row i of sequence b stands at position t = starts[b] + i (lengths[b] - sq + i when starts is 0: the rows are the last
  * ones); the score of key j is s = scale q.k_j, then softcap * tanh(s / softcap) when softcap > 0, then - slopes[h] *
  * |t - j|.  It is seen when all of these hold:
  *   j < lengths[b] (sk when lengths is 0);

@@ -153,7 +153,10 @@ def test_attention_refusals(bridge, buffers):
     refused(sk=9)
     refused(softcap=-1.0)
     refused(softcap=float("inf"))
+    refused(softcap=1e-20)
+    refused(softcap=float("nan"))
     refused(scale=float("nan"))
+    refused(scale=1e30)
     refused(prefixes=i2, causal=False)
     refused(slopes=i16)
     refused(documents=i2)
@@ -403,6 +406,76 @@ def test_attention_of_prompts(bridge, buffers, dtype, d, hq, hkv, s, rule):
     check_attention(bridge, buffers, dtype, b, hq, hkv, s, s, d, spread=3.0, **kw)
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("rule", ["plain", "capped", "biased", "prefix, ragged", "both, negative scale"])
+def test_attention_of_prompts_beyond_one_tile_a_cta(bridge, buffers, dtype, rule):
+    """More than 1024 keys of heads of 64: two query tiles share a CTA and its key tiles."""
+    kw = dict(starts=[0], scale=0.2)
+    if rule == "capped":
+        kw["softcap"] = 8.0
+    if rule == "biased":
+        kw["slopes"] = [0.03, 0.5]
+    if "prefix" in rule:
+        kw.update(prefixes=[300], lengths=[1101])
+    if "both" in rule:
+        kw.update(causal=False, scale=-0.1)
+    check_attention(bridge, buffers, dtype, 1, 2, 1, 1155, 1155, 64, spread=2.0, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_prompts_that_end_in_a_late_tile(bridge, buffers, dtype, d):
+    """NaN and infinities behind lengths that end in the first to the last of many key tiles."""
+    lengths = [1, 129, 300, 511, 640, 777, 901, 1023]
+    check_attention(bridge, buffers, dtype, 8, 1, 1, 1024, 1024, d, lengths=lengths, starts=[0] * 8)
+    check_attention(bridge, buffers, dtype, 8, 1, 1, 200, 1024, d, lengths=lengths, causal=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [1, 3, 8, 24, 104, 112])
+@pytest.mark.parametrize("sq,sk", [(1, 70), (3, 9), (100, 100)])
+def test_attention_unusual_head_sizes(bridge, buffers, dtype, d, sq, sk):
+    check_attention(bridge, buffers, dtype, 2, 3, 3, sq, sk, d, lengths=[sk, sk - 3], starts=[sk - sq, 0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sq", [1, 90])
+def test_attention_with_keys_shared_by_the_batch_and_as_their_own_values(bridge, buffers, dtype, sq):
+    """A batch stride of zero, and one buffer for keys and values."""
+    b, h, sk, d = 3, 2, 90, 64
+    q, k = normal(1, b, h, sq, d), normal(2, 1, h, sk, d)
+    hk = buffers.put(k, dtype)
+    view = HeadView(hk, (0, d, sk * d))
+    out = buffers.own(bridge.decoder_attention(buffers.put(q, dtype), view, view, b, h, h, sq, sk, d, dtype))
+    kr = np.broadcast_to(rounded(k, dtype), (b, h, sk, d))
+    want, err = oracle.attention(rounded(q, dtype), kr, kr, dtype, 1 / 8)
+    within(buffers.get(out, (b, h, sq, d), dtype), want, err)
+
+
+def test_two_bridges_at_once(bridge, buffers):
+    """Calls on two bridges of one device overlap on the GPU; each has its own stream and scratch."""
+    from browsergrad_b200 import CudaBridge
+    other = CudaBridge(0)
+    try:
+        mine, theirs = buffers, Buffers(other)
+        jobs = []
+        for who, bufs in ((bridge, mine), (other, theirs)):
+            q, k, v = normal(len(jobs), 1, 4, 2, 64), normal(7 + len(jobs), 1, 2, 9000, 64), normal(9 + len(jobs), 1, 2, 9000, 64)
+            jobs.append((who, bufs, [bufs.put(x, "bfloat16") for x in (q, k, v)], (q, k, v), []))
+        for _ in range(4):
+            for who, bufs, h, _, outs in jobs:
+                outs.append(bufs.own(who.decoder_attention(*h, 1, 4, 2, 2, 9000, 64, "bfloat16")))
+        for _, bufs, _, (q, k, v), outs in jobs:
+            want, err = oracle.attention(*(rounded(x, "bfloat16") for x in (q, k, v)), "bfloat16", 1 / 8)
+            for o in outs:
+                within(bufs.get(o, (1, 4, 2, 64), "bfloat16"), want, err)
+        for h in theirs.handles:
+            other.release(h)
+        assert other.aliveHandleCount() == 0
+    finally:
+        other.close()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("sq", [1, 4, 200])
 def test_attention_rows_that_see_nothing_are_zero(bridge, buffers, dtype, sq):
@@ -532,6 +605,22 @@ def test_sampling_matches_the_definition(bridge, buffers, dtype, vocab, kw):
     u = np.random.default_rng(vocab).random(n, dtype=np.float32)
     u[0], u[1] = 0.0, np.float32(1 - 2.0 ** -24)
     check_sample(bridge, buffers, logits(vocab, n, vocab), u, dtype, **kw)
+
+
+@pytest.mark.parametrize("top_k", [5, 127, 128, 129, 256, 257, 3000, 39999])
+@pytest.mark.parametrize("top_p", [1.0, 0.6])
+def test_sampling_of_many_ranks(bridge, buffers, top_k, top_p):
+    """From the list of the threads' own maxima to the general threshold, over values with ties at every rank."""
+    x = rounded(logits(9, 3, 40000), "float16")
+    x[1] = np.round(x[1])
+    x[2, 100:] = -np.inf                     # fewer candidates than ranks
+    check_sample(bridge, buffers, x, np.array([0.2, 0.7, 0.95], np.float32), "float16", top_k=top_k, top_p=top_p)
+
+
+def test_sampling_of_a_large_batch(bridge, buffers):
+    """Several rounds of clusters on the device, one and several CTAs a row."""
+    for n, vocab in ((600, 3000), (170, 33001)):
+        check_sample(bridge, buffers, logits(n, n, vocab), np.random.default_rng(n).random(n, dtype=np.float32), "bfloat16", top_p=0.9, top_k=0)
 
 
 @pytest.mark.parametrize("vocab", [64, 5000, 60001])
