@@ -44,24 +44,27 @@ CacheAttnPlan cache_attention_plan(const DecoderAttention& p, int dtype, int sm_
   const long long units = (long long)p.b * p.hkv * ((rows + per_cta - 1) / per_cta);
   // How many CTAs share the keys: the number estimated to take the least time, in keys that an SM slot works through.  A
   // CTA costs its keys and about 384 more (start, join of its groups, partial result), the kernel that joins the splits
-  // about 700.  Sequences of equal length run in whole rounds of CTAs.  Where lengths are given they are taken to differ:
-  // few CTAs then wait for the longest (a third more), three rounds of not too short ones even out.  32 sequences of about
-  // 5000 of 8192 keys, 8 key heads: 155 us in two parts each, 131 us in four; one of 131077, 4 key heads: 94 us in 112
-  // parts, 68 us in the 74 of one round.
-  const double slots = 2.0 * sm_count;
+  // about 700.  Sequences of equal length run in whole rounds of CTAs; with one row tile the memory is the bound, and three
+  // quarters of the slots draw nearly all of it (256 sets of 8192 keys of 128, bf16: 167 us in one part each, 175 in three;
+  // 64 sets of 2048: 35 in one, 21 in four).  Where lengths are given they are taken to differ: few CTAs then wait for the
+  // longest (a third more), three rounds of not too short ones even out (32 sequences of about 5000 of 8192 keys, 8 key
+  // heads: 155 us in two parts each, 128 in six; one of 131077, 4 key heads of two row tiles: 94 us in 112 parts, 65 in the
+  // 74 of one round).
+  const int head = cache_attn::padded_head(p.d);
+  const double slots = (plan.row_tiles == 1 && dtype != BG_F32 && head > 64 && head <= 128 ? 3.0 : 2.0) * sm_count;      // CTAs that run at once
   long long splits = 1, most = (p.sk + 511) / 512;
   if (most > 128) most = 128;
   double best = 1e300;
   for (long long s = 1; s <= most; ++s) {
     const double keys = (double)p.sk / (double)s, cta = keys + 384.0, ctas = (double)(units * s);
-    double t = ceil(ctas / slots) * cta;
-    if (p.lengths) t = ctas >= 3.0 * slots && keys >= 1536.0 ? ctas * cta / slots + 0.25 * cta : 1.3 * t;
+    const double rounds = ceil(ctas / slots);
+    double t = plan.row_tiles == 1 ? fmax(ctas * cta / slots, 0.75 * cta * rounds) : rounds * cta;
+    if (p.lengths) t = ctas >= 3.0 * slots && keys >= 1024.0 ? ctas * cta / slots + 0.25 * cta : 1.3 * rounds * cta;
     if (s > 1) t += 700.0;
     if (t < best) { best = t; splits = s; }
   }
   plan.splits = (int)splits;
   plan.partial_bytes = splits > 1 ? units * splits * per_cta * (cache_attn::padded_head(p.d) + 2) * 4 : 0;
-  (void)dtype;
   return plan;
 }
 

@@ -90,7 +90,9 @@ template <typename T, int DP_, int RT_>
 struct Cfg {
   static constexpr int DP = DP_, RT = RT_, ES = sizeof(T);
   static constexpr int Warps = (RT == 4 && DP <= 128) || DP <= 64 ? 8 : 4;
-  static constexpr int PerSm = 2;                       // CTAs that share an SM (their start and end overlap)
+  // CTAs that share an SM (their start and end overlap).  With one row tile of 16-bit heads above 64 a third one fits when
+  // the ring has two stages: 32 x 8 heads of 8192 keys of 128 at 6.4 TB/s against 6.0; with two row tiles it does not pay.
+  static constexpr int PerSm = DP > 128 ? 1 : ES == 2 && RT == 1 && DP > 64 ? 3 : 2;
   static constexpr int KG = Warps / RT;                 // key groups
   static constexpr int Threads = Warps * 32;
   static constexpr int KT = ES == 2 ? (RT == 1 ? 16 : 32) : (RT == 1 ? 8 : 16);   // keys of a tile
@@ -98,7 +100,7 @@ struct Cfg {
   static constexpr int TileBytes = KT * LD * ES;        // one K or V tile
   static constexpr int SetBytes = KG * 2 * TileBytes;   // a stage of every group
   static constexpr int QBytes = 16 * RT * LD * ES;
-  static constexpr int Stages = RT == 4 ? 2 : (4 * SetBytes + QBytes <= 108 * 1024 ? 4 : 3 * SetBytes + QBytes <= 109 * 1024 ? 3 : 2);
+  static constexpr int Stages = RT == 4 || PerSm == 3 ? 2 : (4 * SetBytes + QBytes <= 108 * 1024 ? 4 : 3 * SetBytes + QBytes <= 109 * 1024 ? 3 : 2);
   static constexpr int MergeLd = DP + 4;
   static constexpr int MergeBytes = Warps * 16 * MergeLd * 4;
   static constexpr int RingBytes = Stages * SetBytes;
@@ -106,7 +108,7 @@ struct Cfg {
 };
 
 template <typename T, int DP, int RT>
-__global__ void __launch_bounds__(Cfg<T, DP, RT>::Threads, DP <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(Cfg<T, DP, RT>::Threads, Cfg<T, DP, RT>::PerSm)
 cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, int row_tiles, int vec, float* partials) {
   using C = Cfg<T, DP, RT>;
   constexpr int KT = C::KT, LD = C::LD, KG = C::KG, ST = C::Stages, ROWS = 16 * RT, GT = RT * 32;
