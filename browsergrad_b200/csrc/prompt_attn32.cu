@@ -10,7 +10,8 @@
 // What differs is what the rules ask: shared key heads, a visible range and a document per row instead of a mask tensor,
 // cap and bias, and value rows behind the sequence's length become zeros as they are converted.  The cap is the library's
 // tanhf: its error is scaled by the cap into the exponent, and fp32 results are held to some 10^-6.
-// Bound: 48 tf32 instructions a tile of 128 x 64, 50 to 65 clocks each.
+// Measured: 8 x 12 heads of 1024 tokens of 64, biased, 119 us (29 us as three tf32 products at half the bf16 rate); the tensor
+// pipe is 25 % busy: products and softmax of the one query tile an SM holds take turns.
 // No cluster multicast; every wait is clock-bounded.
 #include "serving.h"
 
