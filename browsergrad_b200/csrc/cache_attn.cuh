@@ -29,7 +29,6 @@ namespace bg {
 namespace cache_attn {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxPos = 1 << 30;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
@@ -155,7 +154,9 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
       }
     }
     s_hi[tid] = hi;
-    s_pos[tid] = (int)min(max(pos, (long long)-kMaxPos), (long long)kMaxPos);
+    // (for distances alone: moving a row that lies outside the keys up to them adds one number to all its scores, which the
+    // softmax does not see and 32 bits hold better)
+    s_pos[tid] = (int)min(max(pos, 0ll), (long long)len);
     s_doc[tid] = doc;
     if (hi > 0) {
       atomicMax(&s_top, hi);
@@ -540,7 +541,9 @@ few_rows_kernel(const __grid_constant__ DecoderAttention p, int splits, int vec,
       }
     }
     s_hi[tid] = hi;
-    s_pos[tid] = (int)min(max(pos, (long long)-kMaxPos), (long long)kMaxPos);
+    // (for distances alone: moving a row that lies outside the keys up to them adds one number to all its scores, which the
+    // softmax does not see and 32 bits hold better)
+    s_pos[tid] = (int)min(max(pos, 0ll), (long long)len);
     s_doc[tid] = doc;
   }
   for (int i = tid; i < R * DP; i += C::Threads) {

@@ -316,7 +316,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         doc = me.keys > 0 && me.first >= 0 && me.first < a.sk ? __ldg(docs + me.first) : -1;
         if (doc < 0) hi = 0;
       }
-      const int pos = me.first;
+      const int pos = distance_origin(seq, me.first);
       const float slope = BIAS && a.slopes ? a.slopes[h] * kLog2e : 0.f;
       const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_cap = CAP ? a.scale / a.cap : 0.f;
       constexpr bool TURNS = NT == 2 && (C::Alias || CAP || BIAS);      // (4 x 16 heads, 4096 rows: plain scores of heads of 64 are 8 % slower with turns, the others 2 to 9 % faster)

@@ -287,7 +287,7 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
       doc = me.keys > 0 && me.first >= 0 && me.first < a.sk ? __ldg(docs + me.first) : -1;
       if (doc < 0) hi = 0;
     }
-    const int pos = me.first;
+    const int pos = distance_origin(seq, me.first);
     const float slope = BIAS && a.slopes ? a.slopes[h] * kLog2e : 0.f;
     const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_cap = CAP ? a.scale / a.cap : 0.f;
     constexpr bool FOLD = !CAP && !BIAS;             // the scale is applied in the exponent (it is positive then)

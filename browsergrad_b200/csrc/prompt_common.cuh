@@ -47,6 +47,10 @@ __device__ __forceinline__ Sequence sequence_of(const DecoderAttention& a, int b
   return Sequence{len, pre, a.starts ? (long long)st : (long long)len - a.sq};
 }
 
+// The position distances are taken from.  Moving a row that lies outside the keys up to them adds one number to all its
+// scores, which the softmax does not see and 32 bits hold better.
+__device__ __forceinline__ int distance_origin(const Sequence& q, int pos) { return min(max(pos, 0), q.len); }
+
 // Rows [i0, i1] of sequence b: the positions among them that see any key, and how many keys the last of them sees.
 struct Reach {
   int first, last, keys;       // first > last: none

@@ -492,6 +492,23 @@ def test_attention_rows_that_see_nothing_are_zero(bridge, buffers, dtype, sq):
     assert (got == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,group", [(64, 1), (128, 4)])
+@pytest.mark.parametrize("sq", [1, 3, 130])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_attention_bias_of_rows_far_from_their_keys(bridge, buffers, dtype, d, group, sq, softcap):
+    # Behind all keys |t - j| = t - j, ahead of them j - t: moving such rows further adds one number to all their scores,
+    # which the softmax does not see, so their results are those of rows next to the keys, whatever 32 bits make of slope * t.
+    sk, lengths, slopes = 300, [300, 211], np.array(ALIBI[:2 * group], np.float32)
+    kw = dict(causal=False, lengths=lengths, slopes=slopes, softcap=softcap, seed=31)
+    for near, far in (([300, 211], ([300 + 20_000_003, 211 + 900_001], [2 ** 31 - 1 - sq] * 2)), ([1 - sq] * 2, ([-30_000_001 - sq] * 2, [-2 ** 31] * 2))):
+        got, want, err = run_attention(bridge, buffers, dtype, 2, 2 * group, 2, sq, sk, d, starts=near, **kw)
+        within(got, want, err, "next to the keys")
+        for starts in far:
+            moved, _, _ = run_attention(bridge, buffers, dtype, 2, 2 * group, 2, sq, sk, d, starts=starts, **kw)
+            assert np.array_equal(moved, got), starts
+
+
 def test_attention_default_starts_are_the_last_rows(bridge, buffers):
     check_attention(bridge, buffers, "float32", 3, 2, 2, 4, 50, 64, lengths=[50, 4, 2])
     check_attention(bridge, buffers, "bfloat16", 2, 2, 2, 140, 300, 64, lengths=[300, 150])
