@@ -259,7 +259,7 @@ int rotary_append(const Call& c, const bg_head_view* q, const bg_head_view* k, c
   int *st = nullptr, *ct = nullptr;
   if (int rc = vector_of(c, starts, b, BG_I32, "starts", true, &st)) return rc;
   if (int rc = vector_of(c, counts, b, BG_I32, "counts", true, &ct)) return rc;
-  if (!st && (start < 0 || (!ct && start + s > capacity))) return c.error(BG_ERR_INVALID, "the new rows do not fit the cache");
+  if (!st && (start < 0 || start > capacity || (!ct && start > capacity - s))) return c.error(BG_ERR_INVALID, "the new rows do not fit the cache");
   const bg_handle written[3] = {kc->handle, vc->handle, out_view ? out_view->handle : 0};
   const bg_handle read[5] = {q->handle, k->handle, v->handle, starts, counts};
   for (int i = 0; i < 3; ++i) {

@@ -248,16 +248,16 @@ int bg_rotary(bg_context* ctx, const bg_head_view* x, const bg_rotary_spec* spec
 /* One launch for a step's new rows: row s of sequence b has position starts[b] + s (start + s when starts is 0); q is
  * turned into the result, k is turned and stored at row starts[b] + s of k_cache [b, capacity, hkv, d], v is stored there
  * in v_cache.  With counts only the first counts[b] rows of a sequence enter the caches; all other cache rows stay as they
- * were. */
+ * were.  0 <= start <= capacity, and without counts all s rows fit behind it. */
 int bg_rotary_append(bg_context* ctx, const bg_head_view* q, const bg_head_view* k, const bg_head_view* v, const bg_head_view* k_cache,
                      const bg_head_view* v_cache, const bg_rotary_spec* spec, int64_t b, int64_t hq, int64_t hkv, int64_t s,
                      int64_t capacity, int64_t d, int dtype, bg_handle starts, int64_t start, bg_handle counts,
                      const bg_head_view* out_view, bg_handle* out);
 
 /* Attention of sq query rows over sk key rows, hq query heads in groups that share hkv key heads, d <= 256.
- * |scale| <= 1e18; softcap is 0 (none) or in [1e-6, 1e6].  Row i of sequence b stands at position t = starts[b] + i (lengths[b] - sq + i when starts is 0: the rows are the last
- * ones); the score of key j is s = scale q.k_j, then softcap * tanh(s / softcap) when softcap > 0, then - slopes[h] *
- * |t - j|.  It is seen when all of these hold:
+ * |scale| <= 1e18; softcap is 0 (none) or in [1e-6, 1e6].  Row i of sequence b stands at position t = starts[b] + i
+ * (lengths[b] - sq + i when starts is 0: the rows are the last ones); the score of key j is s = scale q.k_j, then
+ * softcap * tanh(s / softcap) when softcap > 0, then - slopes[h] * |t - j|.  It is seen when all of these hold:
  *   j < lengths[b] (sk when lengths is 0);
  *   not causal, or 0 <= t < lengths[b] and (j <= t or j < prefixes[b]);
  *   no documents, or documents[b, t] = documents[b, j] >= 0.

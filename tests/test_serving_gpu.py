@@ -138,6 +138,17 @@ def test_append_refusals(bridge, buffers):
     refused(starts=ids, s=4)
 
 
+@pytest.mark.parametrize("start", [2 ** 63 - 1, 2 ** 63 - 2, 2 ** 62, 2 ** 41])
+@pytest.mark.parametrize("counted", [False, True])
+def test_append_refuses_a_start_no_cache_has(bridge, buffers, start, counted):
+    x = buffers.put(normal(1, 1, 1, 3, 16), "float32")
+    caches = [buffers.put(np.zeros((1, 1, 8, 16), np.float32), "float32") for _ in range(2)]
+    counts = buffers.put(np.zeros(1), "int32") if counted else None
+    with pytest.raises(KernelError) as e:
+        buffers.own(bridge.rotary_append(x, x, x, *caches, RotarySpec(16), 1, 1, 1, 3, 8, 16, "float32", start=start, counts=counts))
+    assert e.value.status == 1, e.value
+
+
 def test_attention_refusals(bridge, buffers):
     q = buffers.put(normal(1, 2, 4, 3, 16), "float32")
     k, v = (buffers.put(normal(s, 2, 2, 8, 16), "float32") for s in (2, 3))
