@@ -577,6 +577,32 @@ def test_attention_length_outside_the_cache_is_reported(bridge, buffers):
     assert np.isfinite(buffers.get(out, (2, 2, 1, 64), "bfloat16")).all()
 
 
+@pytest.mark.parametrize("dtype,apart", [("bfloat16", 1 << 25), ("float32", 1 << 24)])
+@pytest.mark.parametrize("odd", [0, 1])
+def test_caches_beyond_32_bits_of_offsets(bridge, buffers, dtype, apart, odd):
+    # 160 rows `apart` values from each other: the last ones start 5.3 * 10^9 (bfloat16) and 2.7 * 10^9 (float32, 10.7 * 10^9
+    # bytes) values into the buffer.  Only strides differ from the dense cache, so results are its bit for bit, as long as
+    # both take one kernel: an odd offset keeps TMA out, hence the dense cache starts at it too.
+    b, hq, hkv, rows, d = 1, 4, 2, 160, 64
+    q, k, v = (buffers.put(normal(40 + i, b, h, rows, d), dtype) for i, h in ((1, hq), (2, hkv), (3, hkv)))
+    one = buffers.put(normal(44, b, hq, 1, d), dtype)
+    got = []
+    for stride in (hkv * d, apart):
+        caches = []
+        for _ in range(2):
+            h = buffers.own(bridge.alloc((odd + (rows - 1) * stride + hkv * d,), dtype))
+            caches.append(HeadView(h, (0, stride, d), offset=odd))
+        buffers.own(bridge.rotary_append(q, k, v, *caches, RotarySpec(d), b, hq, hkv, rows, rows, d, dtype))
+        turned = buffers.own(bridge.rotary(caches[0], RotarySpec(d), b, hkv, rows, d, dtype, start=7))
+        got.append([buffers.get(turned, (b, hkv, rows, d), dtype)])
+        for rows_q, handle in ((rows, q), (1, one)):
+            out = buffers.own(bridge.decoder_attention(handle, *caches, b, hq, hkv, rows_q, rows, d, dtype))
+            got[-1].append(buffers.get(out, (b, hq, rows_q, d), dtype))
+    for near, far in zip(*got):
+        assert np.isfinite(near).all() and np.abs(near).max() > 0.1
+        assert np.array_equal(near, far)
+
+
 def test_a_refused_length_is_reported_ahead_of_a_plans_bytes(bridge, buffers):
     """A plan that brings its result to the host after a refused call must not hand out bytes computed from it."""
     q, k = buffers.put(normal(1, 1, 1, 1, 64), "float32"), buffers.put(normal(2, 1, 1, 9, 64), "float32")
