@@ -80,11 +80,27 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// cap tanh(x): fp32 results take the library function; for 16-bit ones 1 - 2 / (1 + e^2x) is off by at most a few
-// 2^-24, absolute, which the cap scales to some 10^-5 in the exponent.
-template <typename T> __device__ __forceinline__ float tanh_for(float x) {
-  if (sizeof(T) == 4) return tanhf(x);
-  return 1.0f - __fdividef(2.0f, 1.0f + ex2(x * (2.0f * kLog2e)));
+// tanh(x) for 16-bit results, |x| > 1: 1 - 2 / (1 + e^2x) is off by at most 2^-21, of a value above 0.76.
+__device__ __forceinline__ float tanh_beyond_one(float x) { return 1.0f - __fdividef(2.0f, 1.0f + ex2(x * (2.0f * kLog2e))); }
+// The cap of n scores: scale s / cap in, cap log2(e) tanh of it out.  fp32 results take the library function.  For 16-bit ones
+// the scores nearly always lie within the cap, and then the polynomial serves; else each value takes the form that is
+// accurate relative to it (the other one's error is absolute, and the cap multiplies it into the exponent: 6 % at a cap of 10^6).
+template <typename T, int N> __device__ __forceinline__ void cap_scores(float* x, float to_log2) {
+  if (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_log2 * tanhf(x[i]);
+    return;
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]));
+  if (__all_sync(0xffffffffu, top <= 1.0f)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= to_log2 * tanh_ratio(x[i] * x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_log2 * (fabsf(x[i]) <= 1.0f ? x[i] * tanh_ratio(x[i] * x[i]) : tanh_beyond_one(x[i]));
+  }
 }
 
 template <typename T, int DP_, int RT_>
@@ -351,6 +367,12 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
         for (int e = 0; e < 4; ++e) s[n][e] = ((c[n][0][e] + c[n][1][e]) + (c[n][2][e] + c[n][3][e])) + c[n][4][e];
     }
     // scores -> the exponent's unit (powers of two), rules, maximum
+    const float to_exponent = p.cap > 0.f ? to_cap : to_log2;
+#pragma unroll
+    for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] *= to_exponent;
+    if (p.cap > 0.f) cap_scores<T, KT / 2>(&s[0][0], to_log2);
     float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
     for (int n = 0; n < KT / 8; ++n) {
@@ -365,7 +387,6 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
       for (int e = 0; e < 4; ++e) {
         const int r = e >> 1, kx = key + (e & 1);
         float y = s[n][e];
-        y = p.cap > 0.f ? to_log2 * tanh_for<T>(y * to_cap) : y * to_log2;
         if (p.slopes) y = fmaf(-slope_r[r], fabsf((float)(pos_r[r] - kx)), y);
         const bool seen = kx < hi_r[r] && (!p.documents || kd[e & 1] == doc_r[r]);
         s[n][e] = seen ? y : -CUDART_INF_F;

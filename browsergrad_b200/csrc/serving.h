@@ -75,6 +75,18 @@ struct DecoderAttention {
 constexpr int kDocBlock = 128;
 cudaError_t launch_doc_ranges(const int* documents, int b, int sk, int2* ranges, cudaStream_t s);
 
+#ifdef __CUDACC__
+// tanh(x) / x from z = x^2 <= 1, fitted to a largest relative error of 6.2e-7: what 16-bit attention caps its scores with.
+// Relative, so that a cap far above the scores costs them no digits.
+__device__ __forceinline__ float tanh_ratio(float z) {
+  float p = fmaf(z, -0.003067060373723507f, 0.016743116080760956f);
+  p = fmaf(z, p, -0.051605675369501114f);
+  p = fmaf(z, p, 0.13281433284282684f);
+  p = fmaf(z, p, -0.3332904279232025f);
+  return fmaf(z, p, 0.9999994039535522f);
+}
+#endif
+
 // Key-split kernel (cache_attn.cu): every type and head size up to 256, few rows per key head or many.
 struct CacheAttnPlan {
   int row_tiles;        // 16-row tiles one CTA works on

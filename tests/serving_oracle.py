@@ -130,3 +130,32 @@ def sample(logits, u, temperature, top_k=0, top_p=1.0, min_p=0.0):
     at = int(np.searchsorted(sums, u * sums[-1], side="right"))
     at = min(at, int(np.flatnonzero(w[kept] > 0)[-1]))
     return int(kept[at]), float(w[kept[at]] / sums[-1])
+
+
+def attention_bound(q, k, v, want, dtype, scale, softcap=0.0, smallest=2.0 ** -25, **rules):
+    """``attention``'s bound with two parts held closer, for its result ``want`` without a bias.
+
+    The cap: tanh is off by 2^-20 of its value, whatever the cap.  Up to 1 the odd polynomial is off by 6.2e-7 and its eight
+    operations by 2^-24 each, together below 2^-20; beyond 1 the form 1 - 2 / (1 + e^2x) is off by at most 2^-21 (the
+    quotient lies in [0, 2], division and exponential are good to 2 units), of a value above 0.76.
+    float16: a probability too small for its type is off by ``smallest`` of the largest of its row."""
+    b, hq, sq, d = q.shape
+    group = hq // k.shape[1]
+    k, v = np.repeat(k, group, 1), np.repeat(v, group, 1)
+    seen, _ = visible(b, sq, k.shape[2], rules.get("causal", True), *(rules.get(n) for n in ("lengths", "starts", "prefixes", "documents")))
+    seen = seen[:, None]
+    s = scale * (q @ k.swapaxes(-1, -2))
+    delta = (d + 16) * 2.0 ** -23 * abs(scale) * (np.abs(q) @ np.abs(k).swapaxes(-1, -2))
+    if softcap:
+        s = softcap * np.tanh(s / softcap)
+        delta = delta + 2.0 ** -20 * np.abs(s)
+    delta = delta + 2.0 ** -22 * np.abs(s)
+    p = np.where(seen, np.exp(s - np.where(seen, s, -np.inf).max(-1, keepdims=True, initial=-1e300)), 0.0)
+    total = p.sum(-1, keepdims=True)
+    p = p / np.where(total == 0, 1.0, total)
+    rel = (p * delta).sum(-1, keepdims=True) + k.shape[2] * 2.0 ** -24 + 2.0 ** -21
+    size = np.abs(v)
+    err = (p * (delta + rel + (HALF[dtype] if dtype != "float32" else 0.0))) @ size + HALF[dtype] * np.abs(want)
+    if dtype == "float16":
+        err = err + (smallest * p.max(-1, keepdims=True, initial=0.0) * seen) @ size + 2.0 ** -25
+    return err

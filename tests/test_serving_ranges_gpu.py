@@ -1,0 +1,34 @@
+"""GPU: the serving operators at the ends of what they accept, against ``serving_oracle``."""
+import numpy as np
+import pytest
+
+from tests import serving_oracle as oracle
+from tests.test_serving_gpu import DTYPES, buffers, normal, rounded, within  # noqa: F401  (buffers is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(bridge, buffers, dtype, q, k, v, **rules):
+    """[b, heads, rows, d] arrays through the bridge; index rules are given as arrays."""
+    (b, hq, sq, d), (_, hkv, sk, _) = q.shape, k.shape
+    dev = {n: buffers.put(np.asarray(x), "int32") if n in ("lengths", "starts", "prefixes", "documents") else x for n, x in rules.items()}
+    out = buffers.own(bridge.decoder_attention(*(buffers.put(x, dtype) for x in (q, k, v)), b, hq, hkv, sq, sk, d, dtype, **dev))
+    return buffers.get(out, (b, hq, sq, d), dtype)
+
+
+def expected(dtype, q, k, v, smallest=2.0 ** -25, **rules):
+    q, k, v = (rounded(x, dtype) for x in (q, k, v))
+    scale = rules.pop("scale", 1 / np.sqrt(q.shape[-1]))
+    want, _ = oracle.attention(q, k, v, dtype, scale, **rules)
+    return want, oracle.attention_bound(q, k, v, want, dtype, scale, smallest=smallest, **rules)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq", [1, 63, 64, 200])
+@pytest.mark.parametrize("softcap", [1e3, 1e5, 1e6])
+def test_attention_caps_far_above_the_scores(bridge, buffers, dtype, d, sq, softcap):
+    """A cap that hardly bends the scores must not cost them their digits."""
+    q, k, v = normal(1, 2, 4, sq, d) * 1.5, normal(2, 2, 2, 300, d), normal(3, 2, 2, 300, d)
+    rules = dict(lengths=[300, 211], softcap=softcap)
+    within(attend(bridge, buffers, dtype, q, k, v, **rules), *expected(dtype, q, k, v, **rules))
