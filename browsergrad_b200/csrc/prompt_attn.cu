@@ -365,7 +365,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             else z0 = fmax3(z0, fabsf(x[i]), fabsf(x[i + 1]));
           }
           if (__all_sync(0xffffffffu, fmaxf(z0, z1) <= 1.0f)) {
-            // tanh(x) = x P(x^2) on [-1, 1], fitted to a largest relative error of 6.2e-7
+            // tanh_ratio, two values an instruction
 #pragma unroll
             for (int i = 0; i < kKeys; i += 2) {
               float z, y, q, r;
@@ -379,9 +379,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
               mul2(x[i], x[i + 1], x[i], x[i + 1], q, r);
             }
           } else {
+            // A score beyond the cap among them, or whatever lies behind the sequence's keys: each value takes the form that is
+            // accurate relative to it, the polynomial with the very operations of the block above, so that a score's bits do not
+            // depend on its neighbours.
 #pragma unroll
             for (int i = 0; i < kKeys; ++i)
-              x[i] = to_log2 * (1.0f - __fdividef(2.0f, 1.0f + ex2_approx(x[i] * (2.0f * kLog2e))));
+              x[i] = fabsf(x[i]) <= 1.0f ? x[i] * to_log2 * tanh_ratio(x[i] * x[i])
+                                         : to_log2 * (1.0f - __fdividef(2.0f, 1.0f + ex2_approx(x[i] * (2.0f * kLog2e))));
           }
         } else if (BIAS) {
 #pragma unroll

@@ -32,3 +32,35 @@ def test_attention_caps_far_above_the_scores(bridge, buffers, dtype, d, sq, soft
     q, k, v = normal(1, 2, 4, sq, d) * 1.5, normal(2, 2, 2, 300, d), normal(3, 2, 2, 300, d)
     rules = dict(lengths=[300, 211], softcap=softcap)
     within(attend(bridge, buffers, dtype, q, k, v, **rules), *expected(dtype, q, k, v, **rules))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("sq", [9, 64, 200])
+def test_attention_rows_beyond_the_cap_next_to_rows_far_below_it(bridge, buffers, dtype, sq):
+    """Every eighth row's scores pass the cap (their exponents are off by about one in 32 bits: only finite), the others are a
+    millionth of it and keep their digits."""
+    q, k, v = normal(1, 1, 2, sq, 64), normal(2, 1, 2, 300, 64), normal(3, 1, 2, 300, 64)
+    q[:, :, ::8] *= 1e7
+    rules = dict(softcap=1e6, causal=False)
+    got, (want, err) = attend(bridge, buffers, dtype, q, k, v, **rules), expected(dtype, q, k, v, **rules)
+    assert np.isfinite(got).all()
+    low = np.arange(sq) % 8 != 0
+    within(got[:, :, low], want[:, :, low], err[:, :, low])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq", [1, 64, 200])
+@pytest.mark.parametrize("softcap", [0.0, 30.0, 1e3])
+@pytest.mark.parametrize("sk", [200, 1300])
+def test_attention_does_not_see_what_a_cache_holds_behind_a_length(bridge, buffers, dtype, d, sq, softcap, sk):
+    """Results are the same bit for bit whatever lies behind the length: zeros, large numbers, infinities or NaN."""
+    lengths = [sk - 5, sk - 150, 1]
+    q, k, v = normal(1, 3, 4, sq, d), normal(2, 3, 2, sk, d), normal(3, 3, 2, sk, d)
+    got = []
+    for behind in (0.0, 3e4, -np.inf, np.nan):
+        for i, n in enumerate(lengths):
+            k[i, :, n:], v[i, :, n:] = behind, behind
+        got.append(attend(bridge, buffers, dtype, q, k, v, lengths=lengths, starts=[0, 3, 0], softcap=softcap, causal=sq > 64))
+    for other in got[1:]:
+        assert np.array_equal(got[0], other)
