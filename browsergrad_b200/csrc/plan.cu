@@ -3523,8 +3523,8 @@ std::shared_ptr<CompiledPlan> Compiler::compile() {
 
 }  // namespace
 
-// Reads (and clears) the status word as last copied to the host; call after a synchronisation of the stream, or
-// without one to pick up what an earlier copy already delivered.
+// Reads (and clears) the status word as last copied to the host; call after a synchronisation of the stream: work in flight
+// may write the word again, and the next valid call would be blamed for it.
 int take_device_status(bg_context* ctx) {
   ctx->status_pending = false;
   const int st = *ctx->h_status;
@@ -3533,6 +3533,12 @@ int take_device_status(bg_context* ctx) {
     cudaMemsetAsync(ctx->d_status, 0, sizeof(int), ctx->stream);
   }
   return st;
+}
+
+int take_early_status(bg_context* ctx) {
+  if (!ctx->status_pending || *(volatile int*)ctx->h_status == 0) return 0;
+  if (cudaStreamSynchronize(ctx->stream) != cudaSuccess) return 0;      // (the caller's own next CUDA call reports that)
+  return take_device_status(ctx);
 }
 
 std::string device_status_message(int status_rc) {
@@ -3547,10 +3553,7 @@ int run_plan(bg_context* ctx, const bg_plan* plan, const bg_plan_input* inputs, 
   if (n_inputs > 0 && !inputs) return fail(ctx, BG_ERR_INVALID, "run_tensor_plan: null inputs");
   cudaSetDevice(ctx->device);
   // a device-side wait that gave up in an earlier plan whose root stayed on the device is reported here at the latest
-  if (ctx->status_pending && *ctx->h_status != 0) {
-    const int st = take_device_status(ctx);
-    return fail(ctx, st, device_status_message(st) + " (in an earlier plan)");
-  }
+  if (const int st = take_early_status(ctx)) return fail(ctx, st, device_status_message(st) + " (in an earlier plan)");
   uint64_t h = 1469598103934665603ull;
   h = fnv1a(plan->steps, sizeof(bg_plan_step) * (size_t)plan->n_steps, h);
   if (plan->n_ext > 0) h = fnv1a(plan->ext, sizeof(int32_t) * (size_t)plan->n_ext, h);

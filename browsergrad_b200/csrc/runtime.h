@@ -108,6 +108,9 @@ void* cast_copy_for(bg_context* ctx, const void* ptr, int64_t bytes, int dtype, 
 void cast_copy_drop(bg_context* ctx, const void* ptr);
 
 int take_device_status(bg_context* ctx);
+// The same ahead of new work, without waiting as long as nothing has been reported: 0, or the status of earlier work, whose
+// stream has then been synchronised.
+int take_early_status(bg_context* ctx);
 std::string device_status_message(int status_rc);
 int run_plan(bg_context* ctx, const bg_plan* plan, const bg_plan_input* inputs, int n_inputs, void* out_host,
              size_t out_nbytes, bg_handle* out_handle);

@@ -2,6 +2,8 @@
 import numpy as np
 import pytest
 
+from browsergrad_b200 import HeadView
+from browsergrad_b200.errors import KernelError
 from tests import serving_oracle as oracle
 from tests.test_serving_gpu import DTYPES, buffers, normal, rounded, within  # noqa: F401  (buffers is a fixture)
 
@@ -64,3 +66,46 @@ def test_attention_does_not_see_what_a_cache_holds_behind_a_length(bridge, buffe
         got.append(attend(bridge, buffers, dtype, q, k, v, lengths=lengths, starts=[0, 3, 0], softcap=softcap, causal=sq > 64))
     for other in got[1:]:
         assert np.array_equal(got[0], other)
+
+
+def refuse_for_long(bridge, buffers):
+    """A call whose every CTA reports its length, waves of them one after another: 2048 sequences of one long cache."""
+    b, h, sk, d = 2048, 8, 16384, 128
+    q = buffers.put(np.zeros((b, h, 1, d), np.float32), "bfloat16")
+    k = buffers.put(np.zeros((1, h, sk, d), np.float32), "bfloat16")
+    n = buffers.put(np.full(b, sk + 1), "int32")
+    view = HeadView(k, (0, d, sk * d))
+    bridge.synchronize()
+    return buffers.own(bridge.decoder_attention(q, view, view, b, h, h, 1, sk, d, "bfloat16", lengths=n))
+
+
+@pytest.mark.parametrize("who", ["serving call", "plan"])
+def test_a_refusal_in_flight_is_reported_once(bridge, buffers, who):
+    """The refused call still runs, and still reports, when the next call learns of it; a valid call after that one succeeds."""
+    x = normal(1, 1, 1, 256, 256)
+    h = buffers.put(x, "float32")
+    call = {"serving call": lambda: bridge.decoder_attention(h, h, h, 1, 1, 1, 256, 256, 256, "float32"),
+            "plan": lambda: bridge.matmul(h, h, 256, 256, 256, "float32")}[who]
+    for _ in range(3):
+        refuse_for_long(bridge, buffers)
+        with pytest.raises(KernelError) as e:
+            while True:                                   # until the first report has crossed to the host
+                buffers.own(call())
+        assert e.value.status == 7
+        got = buffers.get(buffers.own(call()), x.shape, "float32")
+        assert np.isfinite(got).all() and np.abs(got).max() > 0
+        bridge.synchronize()
+
+
+def test_two_refused_calls_in_flight_leave_the_next_valid_one_alone(bridge, buffers):
+    x = normal(1, 1, 2, 3, 64)
+    h = buffers.put(x, "float32")
+    n = buffers.put(np.array([4]), "int32")
+    for _ in range(3):
+        refuse_for_long(bridge, buffers)
+        with pytest.raises(KernelError) as e:
+            while True:
+                buffers.own(bridge.decoder_attention(h, h, h, 1, 2, 2, 3, 3, 64, "float32", lengths=n))
+        assert e.value.status == 7
+        out = buffers.own(bridge.decoder_attention(h, h, h, 1, 2, 2, 3, 3, 64, "float32"))
+        assert np.isfinite(buffers.get(out, x.shape, "float32")).all()
