@@ -7,6 +7,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <map>
+#include <mutex>
 
 #include "runtime.h"
 
@@ -442,6 +444,20 @@ int guarded(bg_context* ctx, const char* op, bg_handle* out, F&& fn) {
 }
 
 }  // namespace
+
+cudaError_t allow_shared(const void* kern, size_t bytes) {
+  static std::mutex lock;
+  static std::map<std::pair<int, const void*>, size_t> limits;
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  std::lock_guard<std::mutex> hold(lock);
+  size_t& limit = limits[{dev, kern}];
+  if (limit >= bytes) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) limit = bytes;
+  return e;
+}
+
 }  // namespace bg
 
 using namespace bg;

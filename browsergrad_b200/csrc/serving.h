@@ -17,21 +17,12 @@ struct StatusWords {
   int* host;
 };
 
-// Raises a kernel's limit of dynamic shared memory, once per kernel and device (the call costs about a microsecond).
-template <typename K>
-cudaError_t allow_shared(K kern, size_t bytes) {
-  struct Done { int device; size_t bytes; };
-  thread_local std::unordered_map<const void*, std::vector<Done>> done;      // a context is used from one thread at a time
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  auto& v = done[reinterpret_cast<const void*>(kern)];
-  for (auto& d : v)
-    if (d.device == dev && d.bytes >= bytes) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e == cudaSuccess) v.push_back({dev, bytes});
-  return e;
-}
+// Raises a kernel's limit of dynamic shared memory where it is below `bytes`, which is remembered (the call costs about a
+// microsecond).  The limit belongs to the kernel on its device and is shared by all threads and contexts: it is never
+// lowered, and the lock is held across the change, so that a larger one of another thread is not overwritten.
+cudaError_t allow_shared(const void* kern, size_t bytes);
+template <typename... Args>
+cudaError_t allow_shared(void (*kern)(Args...), size_t bytes) { return allow_shared(reinterpret_cast<const void*>(kern), bytes); }
 
 // ---- rotary.cu ---------------------------------------------------------------------------------------------------
 constexpr int kRotaryMaxPairs = 128;

@@ -1,4 +1,6 @@
 """GPU: the serving operators at the ends of what they accept, against ``serving_oracle``."""
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 
@@ -109,3 +111,27 @@ def test_two_refused_calls_in_flight_leave_the_next_valid_one_alone(bridge, buff
         assert e.value.status == 7
         out = buffers.own(bridge.decoder_attention(h, h, h, 1, 2, 2, 3, 3, 64, "float32"))
         assert np.isfinite(buffers.get(out, x.shape, "float32")).all()
+
+
+def test_a_small_call_of_another_thread_leaves_a_large_one_its_shared_memory(bridge, buffers):
+    """One bridge moves from thread to thread, each call behind the one before it: the limit of a kernel's shared memory is the
+    device's, not the thread's."""
+    u = buffers.put(np.full(2, 0.5, np.float32), "float32")
+    rows = {n: normal(n, 2, n) for n in (1000, 200003)}
+    dev = {n: buffers.put(x, "float32") for n, x in rows.items()}
+    keys = {n: buffers.put(normal(n, 1, 1, n, 128), "bfloat16") for n in (200, 40000)}
+    q = buffers.put(normal(5, 1, 1, 100, 128), "bfloat16")
+
+    def calls(vocab, sk):
+        out = buffers.own(bridge.sample_tokens(dev[vocab], u, 2, vocab, "float32"))
+        att = buffers.own(bridge.decoder_attention(q, keys[sk], keys[sk], 1, 1, 1, 100, sk, 128, "bfloat16"))
+        return buffers.get(out, (2,), "int64"), buffers.get(att, (1, 1, 100, 128), "bfloat16")
+
+    with ThreadPoolExecutor(1) as one, ThreadPoolExecutor(1) as two:
+        first = one.submit(calls, 200003, 40000).result()
+        small = two.submit(calls, 1000, 200).result()
+        again = one.submit(calls, 200003, 40000).result()
+        assert np.array_equal(two.submit(calls, 1000, 200).result()[1], small[1])
+    for a, b in zip(first, again):
+        assert np.array_equal(a, b)
+    assert list(first[0]) == [oracle.sample(r, 0.5, np.float32(1.0))[0] for r in rows[200003]]
