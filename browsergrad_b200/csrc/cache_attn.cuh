@@ -13,7 +13,8 @@
 // keys are also split over CTAs, whose partial results a second kernel joins in split order, a CTA per row.
 // fp32 operands are multiplied as three tf32 products (hi hi + hi lo + lo hi); each tile's P V starts from zero and is
 // added to O in registers, because the tensor core's own accumulation truncates.  16-bit P is rounded to the operand
-// type: each probability is off by at most 2^-8 (bf16) or 2^-11 (f16) of itself, the half step the result is rounded by too.
+// type, because the tensor core multiplies two operands of one type: each probability is off by at most 2^-8 (bf16) or 2^-11
+// (f16) of itself, the half step the result is rounded by too; f16 ones below 2^-28 of the largest by up to 2^-39 of it.
 // Measured: 32 x 8 key heads of 8192 keys of 128, bf16, 167 us = 6.4 TB/s; 131077 keys, 4 key heads of two row tiles, f16,
 // 65 us (41 us at the copy rate; 8 warps an SM wait for their own tile's products and exponentials, DRAM 57 % busy);
 // 64 x 12 heads of 2048 keys of 64, fp32, 130 us = 6.2 TB/s; fp32 prompts of heads of 128 (2 x 16 x 2048, causal) 42 TFLOP/s.
@@ -102,6 +103,14 @@ template <typename T, int N> __device__ __forceinline__ void cap_scores(float* x
     for (int i = 0; i < N; ++i) x[i] = to_log2 * (fabsf(x[i]) <= 1.0f ? x[i] * tanh_ratio(x[i] * x[i]) : tanh_beyond_one(x[i]));
   }
 }
+
+// The reference of the exponentials of scores of at most mx.  float16 probabilities lie up to 2^14 above it, where the type has
+// its room: against a reference of mx itself they would lose bits from 2^-14 on and vanish at 2^-25, while their sum below the
+// line still counted them (131077 keys 2^-26 below the largest add up to 2^-9 of it).  Scores from 2^21 on, which 32 bits
+// hold to a quarter, keep mx: the difference would be rounded into the exponent.  The running reference is the largest of the tiles', so no
+// exponent passes 14; sums, rescaling and joins are relative to it, and it cancels in the division.
+template <typename T> __device__ __forceinline__ float below(float mx) { return mx; }
+template <> __device__ __forceinline__ float below<__half>(float mx) { return fabsf(mx) < 2097152.0f ? mx - 14.0f : mx; }
 
 template <typename T, int DP_, int RT_>
 struct Cfg {
@@ -398,6 +407,7 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
     for (int r = 0; r < 2; ++r) {
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+      mx[r] = below<T>(mx[r]);
       const float m_new = fmaxf(m_r[r], mx[r]);
       m_use[r] = m_new == -CUDART_INF_F ? 0.f : m_new;
       alpha[r] = ex2(m_r[r] - m_use[r]);

@@ -12,7 +12,9 @@
 // With 64 values a head P has columns of its own in tensor memory, and the scores of the next key tile are computed
 // while a tile's softmax still runs; with 128 values the 512 columns are S and O of both tiles, P takes the place of the
 // scores it was made from, and the next scores wait for P V.  The reference of the exponentials follows the row maximum
-// lazily: O is rescaled when the maximum has grown by more than 2^8.
+// lazily: O is rescaled when the maximum has grown by more than 2^8.  P is rounded to the operand type, which is what the
+// tensor core multiplies: each probability is off by at most 2^-8 (bf16) or 2^-11 (f16) of itself, f16 ones below 2^-21 of the
+// reference (kRoomF16) by up to 2^-32 of it.
 // Which keys a row sees is one number, the end of its visible range, and for packed documents the row's id: tiles nobody
 // sees are not loaded, tiles everybody sees are not masked, for the rest the bits of the keys seen are made while the
 // tile's scores are (packed documents of 4 x 2048: 53 us with a pass over the scores, 49 this way).
@@ -46,6 +48,9 @@ using attn::tma_load_4d;
 constexpr int kRows = 128, kKeys = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyLog2 = 8.0f;
+// float16 probabilities lie up to 2^7 above the reference, 2^15 with the lazy maximum, where the type still has room: against
+// the maximum itself they would vanish below 2^-25 of it while their sum still counted them.  It cancels in the division.
+constexpr float kRoomF16 = 7.0f;
 // D: values of a head, padded; NT: query tiles of a CTA.
 template <int D, int NT>
 struct Cfg {
@@ -422,6 +427,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (FOLD) mt *= to_log2;
           else mt += base;
+          if (!BF16 && fabsf(mt) < 2097152.0f) mt -= kRoomF16;      // (larger ones: 32 bits would round it into the exponent)
         }
         // O is rescaled by whole warps once the P V before it has completed (with P in the place of the scores these
         // scores are younger than that product)

@@ -135,3 +135,54 @@ def test_a_small_call_of_another_thread_leaves_a_large_one_its_shared_memory(bri
     for a, b in zip(first, again):
         assert np.array_equal(a, b)
     assert list(first[0]) == [oracle.sample(r, 0.5, np.float32(1.0))[0] for r in rows[200003]]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sq,group", [(1, 1), (1, 4), (4, 8), (64, 1), (130, 1)])
+@pytest.mark.parametrize("at", [0, 70000, 131077])
+def test_attention_keeps_what_many_small_probabilities_add_up_to(bridge, buffers, dtype, sq, group, at):
+    """One key 18 above 131077 others: each of those has a probability of 2^-26, below what float16 holds beside a largest one
+    of 1, and together they have 2^-9.  The largest key's value is zero, so that they are the whole result."""
+    sk, d = 131078, 64
+    q, k, v = np.zeros((1, group, sq, d), np.float32), np.zeros((1, 1, sk, d), np.float32), np.ones((1, 1, sk, d), np.float32)
+    q[..., 0], k[:, :, at, 0], v[:, :, at] = 1.0, 18.0, 0.0
+    rules = dict(scale=1.0, causal=False)
+    want = np.full(q.shape, (sk - 1) / (sk - 1 + np.exp(18.0)))
+    # scores are exact; a probability is rounded relatively (HALF), in float16 by at least half its smallest step, 2^-25 of a
+    # reference that lies at most 2^7 below the largest; the sums over the keys (32 bits, n terms) and the exponential as in attention()
+    err = want * (2 * oracle.HALF[dtype] + 2 * (sk * 2.0 ** -24 + 2.0 ** -21)) + (sk * 2.0 ** -32 if dtype == "float16" else 0.0)
+    within(attend(bridge, buffers, dtype, q, k, v, **rules), want, err)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [1, 4, 24])
+def test_attention_keeps_small_probabilities_of_unsplit_caches(bridge, buffers, dtype, group):
+    """The same for a batch so large that no sequence's keys are split over CTAs: the warps that do not meet the largest key have
+    references of their own, the one that does holds a part of the others."""
+    b, sk, d = 300, 16384, 64
+    q, k, v = np.zeros((b, group, 1, d), np.float32), np.zeros((1, 1, sk, d), np.float32), np.ones((1, 1, sk, d), np.float32)
+    q[..., 0], k[:, :, 0, 0], v[:, :, 0] = 1.0, 18.0, 0.0
+    views = [HeadView(buffers.put(x, dtype), (0, d, sk * d)) for x in (k, v)]
+    out = buffers.own(bridge.decoder_attention(buffers.put(q, dtype), *views, b, group, 1, 1, sk, d, dtype, scale=1.0, causal=False))
+    want = np.full(q.shape, (sk - 1) / (sk - 1 + np.exp(18.0)))
+    err = want * (2 * oracle.HALF[dtype] + 2 * (sk * 2.0 ** -24 + 2.0 ** -21)) + (sk * 2.0 ** -32 if dtype == "float16" else 0.0)
+    within(buffers.get(out, q.shape, dtype), want, err)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("sq", [1, 64, 200])
+@pytest.mark.parametrize("size,factor", [(3.0, 1.0), (300.0, 1.0), (6e4, 1.0), (6e4, 10.0), (6e4, 50.0)])
+def test_attention_of_16_bits_with_large_scores_stays_finite(bridge, buffers, dtype, sq, size, factor):
+    """Scores from tens to 2.4 * 10^7 of either sign, which rise and fall along the keys: no probability passes its type."""
+    sk, d = 700, 64
+    q, k, v = np.ones((1, 2, sq, d), np.float32), np.zeros((1, 2, sk, d), np.float32), normal(3, 1, 2, sk, d)
+    k[..., 0] = np.linspace(-1, 1, sk) * size
+    k[:, 1] = k[:, 1, ::-1]
+    q[..., 0] = factor
+    rules = dict(scale=8.0, causal=False)
+    got = attend(bridge, buffers, dtype, q, k, v, **rules)
+    assert np.isfinite(got).all()
+    if size < 1e3:
+        within(got, *expected(dtype, q, k, v, **rules))
+    else:                                      # 32 bits leave the exponents no digits; the largest key still takes nearly all
+        assert np.abs(got).max() <= np.abs(rounded(v, dtype)).max() * (1 + 2.0 ** -6)
