@@ -100,7 +100,7 @@ template <typename T, int N> __device__ __forceinline__ void cap_scores(float* x
     for (int i = 0; i < N; ++i) x[i] *= to_log2 * tanh_ratio(x[i] * x[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_log2 * (fabsf(x[i]) <= 1.0f ? x[i] * tanh_ratio(x[i] * x[i]) : tanh_beyond_one(x[i]));
+    for (int i = 0; i < N; ++i) x[i] = to_log2 * within_one(x[i] * x[i], x[i] * tanh_ratio(x[i] * x[i]), tanh_beyond_one(x[i]));
   }
 }
 

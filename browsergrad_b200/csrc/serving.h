@@ -76,6 +76,12 @@ __device__ __forceinline__ float tanh_ratio(float z) {
   p = fmaf(z, p, -0.3332904279232025f);
   return fmaf(z, p, 0.9999994039535522f);
 }
+// `within` where z <= 1, else `beyond`: a selection between two values at hand (a branch for each score would diverge).
+__device__ __forceinline__ float within_one(float z, float within, float beyond) {
+  float y;
+  asm("{\n\t.reg .pred p;\n\tsetp.le.f32 p, %1, 0f3F800000;\n\tselp.f32 %0, %2, %3, p;\n\t}" : "=f"(y) : "f"(z), "f"(within), "f"(beyond));
+  return y;
+}
 #endif
 
 // Key-split kernel (cache_attn.cu): every type and head size up to 256, few rows per key head or many.
