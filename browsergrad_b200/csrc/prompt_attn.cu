@@ -474,13 +474,20 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (FOLD) mt *= to_log2;
           else mt += base;
-          if (!BF16 && fabsf(mt) < 2097152.0f) mt -= kRoomF16;      // (larger ones: 32 bits would round it into the exponent)
         }
+        const bool coarse = fabsf(mt) >= kCoarse && mt != -CUDART_INF_F;
+        if (!BF16 && !coarse) mt -= kRoomF16;
         // O is rescaled by whole warps once the P V before it has completed (with P in the place of the scores these
         // scores are younger than that product)
         bool pv_done = t == 0 || C::Alias;
         const bool raise = m_ref != -CUDART_INF_F && mt - m_ref > kLazyLog2;
-        if (__any_sync(0xffffffffu, raise)) {
+        float unit = to_log2;                               // FOLD: what the scores are still to be multiplied by
+        if (FOLD ? __any_sync(0xffffffffu, raise || coarse) : __any_sync(0xffffffffu, raise)) {
+          if (FOLD && __any_sync(0xffffffffu, coarse)) {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) x[i] *= to_log2;
+            unit = 1.0f;
+          }
           if (!pv_done) {
             ok = __all_sync(0xffffffffu, mbar_wait(&pv_full[g], (uint32_t)(t - 1) & 1u, abort_flag));
             if (!ok) break;
@@ -502,7 +509,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         {
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
           auto exponentials = [&](int i) {                 // of x[i], x[i + 1]
-            if (FOLD) fma2(x[i], x[i + 1], x[i], x[i + 1], to_log2, to_log2, off, off);
+            if (FOLD) fma2(x[i], x[i + 1], x[i], x[i + 1], unit, unit, off, off);
             else add2(x[i], x[i + 1], x[i], x[i + 1], off, off);
             x[i] = ex2_approx(x[i]);
             x[i + 1] = ex2_approx(x[i + 1]);

@@ -363,6 +363,7 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if (FOLD) mt *= to_log2;
       }
+      const bool coarse = FOLD && fabsf(mt) >= kCoarse && mt != -CUDART_INF_F;
       // Chunk boundary: O is folded into registers before this tile's P V starts a fresh accumulator.
       bool o_quiet = t == 0;
       if (t > 0 && (t % kChunkTiles) == 0) {
@@ -373,7 +374,13 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         o_quiet = true;
       }
       const bool raise = m_ref != -CUDART_INF_F && mt - m_ref > kLazyLog2;
-      if (__any_sync(0xffffffffu, raise)) {
+      float unit = to_log2;                           // FOLD: what the scores are still to be multiplied by
+      if (__any_sync(0xffffffffu, raise || coarse)) {
+        if (FOLD && __any_sync(0xffffffffu, coarse)) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) x[i] *= to_log2;
+          unit = 1.0f;
+        }
         const float alpha = raise ? ex2_approx(m_ref - mt) : 1.0f;
         if ((t % kChunkTiles) != 0) {                // the current chunk holds products: they must be complete
           if (!o_quiet) {
@@ -394,7 +401,7 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < kKeys; ++i) {
-          x[i] = ex2_approx(FOLD ? fmaf(x[i], to_log2, off) : x[i] + off);
+          x[i] = ex2_approx(FOLD ? fmaf(x[i], unit, off) : x[i] + off);
           ps[i & 3] += x[i];
         }
         l += (ps[0] + ps[1]) + (ps[2] + ps[3]);

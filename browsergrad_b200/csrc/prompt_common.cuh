@@ -16,6 +16,10 @@ cudaError_t launch_prompt_attention32(const DecoderAttention& p, cudaStream_t s)
 namespace prompt {
 
 constexpr int kMaxPos = 1 << 30;
+// Scores (in powers of two) from here on are a quarter or more apart in 32 bits.  The reference of their exponentials is then the
+// largest of the rounded scores: an unrounded product, what the exponent takes otherwise, may lie half a step above it, and
+// the exponential of that would pass the type (float16 from scores of 2^27 on).
+constexpr float kCoarse = 2097152.0f;
 
 // Bits of the keys (of `keys` that exist from docs on) whose document is this lane's.  Each key's id is read once per warp;
 // the rows of a warp belong to few documents, so the words are made per document, by ballots, not per row.

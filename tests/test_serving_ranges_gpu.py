@@ -169,20 +169,23 @@ def test_attention_keeps_small_probabilities_of_unsplit_caches(bridge, buffers, 
     within(buffers.get(out, q.shape, dtype), want, err)
 
 
-@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("sq", [1, 64, 200])
-@pytest.mark.parametrize("size,factor", [(3.0, 1.0), (300.0, 1.0), (6e4, 1.0), (6e4, 10.0), (6e4, 50.0)])
-def test_attention_of_16_bits_with_large_scores_stays_finite(bridge, buffers, dtype, sq, size, factor):
-    """Scores from tens to 2.4 * 10^7 of either sign, which rise and fall along the keys: no probability passes its type."""
-    sk, d = 700, 64
+@pytest.mark.parametrize("size,factor", [(3.0, 1.0), (300.0, 1.0), (6e4, 1.0), (6e4, 50.0), (6e4, 1e3), (6e4, 2e4), (6e4, 1e19)])
+def test_attention_with_large_scores_stays_finite(bridge, buffers, dtype, d, sq, size, factor):
+    """Scores from tens to 10^24 of either sign, which rise along the keys of one head and fall along the other's: no
+    probability passes its type, and where 32 bits leave the exponents no digits the results are averages of values still."""
+    sk = 700
     q, k, v = np.ones((1, 2, sq, d), np.float32), np.zeros((1, 2, sk, d), np.float32), normal(3, 1, 2, sk, d)
     k[..., 0] = np.linspace(-1, 1, sk) * size
     k[:, 1] = k[:, 1, ::-1]
-    q[..., 0] = factor
-    rules = dict(scale=8.0, causal=False)
+    rules = dict(scale=8.0 * min(factor, 1e17), causal=False)
+    q *= max(factor / 1e17, 1.0)
     got = attend(bridge, buffers, dtype, q, k, v, **rules)
     assert np.isfinite(got).all()
     if size < 1e3:
         within(got, *expected(dtype, q, k, v, **rules))
-    else:                                      # 32 bits leave the exponents no digits; the largest key still takes nearly all
-        assert np.abs(got).max() <= np.abs(rounded(v, dtype)).max() * (1 + 2.0 ** -6)
+    else:
+        top = np.abs(rounded(v, dtype)).max()
+        assert np.abs(got).max() <= top * (1 + 2.0 ** -6) and np.abs(got).max(-1).min() > 1e-3
