@@ -11,9 +11,10 @@
 // until equal values are left, which are taken in index order.  For a small k the histogram is of the threads' own maxima:
 // the buckets that hold k of those hold the k largest values, which are collected, and the rest of the work is comparing
 // all pairs of them.
-// Weights are whole numbers, round(w 2^46) (fewer bits for a vocabulary whose sum would pass 2^62): sums are then exact,
-// the same in any order, so atomics cannot change the result.  A weight is off by at most 2^-46 of the largest and a
-// running sum by some 2^-46 sqrt(V), while u has 24 bits.  The
+// Weights are whole numbers, round(w 2^b), b = 46 below 2^18 tokens and one less from each doubling on (their sum stays below
+// 2^64): sums are then exact, the same in any order, so atomics cannot change the result.  A weight is off by at most 2^-(b+1)
+// of the largest (one below that is nothing) and a running sum by V of those: 2^-30 for 128000 tokens, 2^-24 for 2^20, which is
+// the step of u; longer rows are refused.  The
 // exponential is 64-bit: 2^y = 2^(i / 256) (from a table) e^t, |t| <= ln 2 / 512, the last factor by its series to t^4
 // (4 * 10^-17 dropped): ten 64-bit operations.
 // Bound: barriers between the phases and the latency behind them; the 64-bit pipe is 12 %, the issue slots 37 %, DRAM 2 %
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // ---- read the slice; every thread's largest value ----
   float mine = -CUDART_INF_F;
   for (int i = tid; i < kBuckets; i += kThreads) { sh.low[i] = 0u; sh.high[i] = 0u; }
-  const int bits = min(46, 62 - (64 - __clzll((long long)p.vocab)));
+  const int bits = min(46, __clzll((long long)p.vocab));      // vocab 2^bits < 2^64
   if (tid < 256) sh.table[tid] = exp2((double)tid / 256.0) * (double)(1ull << bits);
   if (tid == 0) sh.n_listed = 0u;
 #pragma unroll 4

@@ -377,6 +377,7 @@ int sample_tokens(const Call& c, bg_handle logits, bg_handle uniforms, int64_t n
   if (int rc = check_type(c, dtype)) return rc;
   if (int rc = check_extent(c, n, 0, "rows")) return rc;
   if (int rc = check_extent(c, vocab, 1, "vocabulary")) return rc;
+  if (vocab > kSampleMaxVocab) return c.error(BG_ERR_UNSUPPORTED, "vocabularies above 1048576");
   if (!(sp->temperature >= 0.0) || !std::isfinite(sp->temperature)) return c.error(BG_ERR_INVALID, "temperature must be zero (greedy) or positive");
   if (sp->top_k < 0) return c.error(BG_ERR_INVALID, "top_k must be zero (all) or positive");
   if (std::isnan(sp->top_p)) return c.error(BG_ERR_INVALID, "top_p is not a number");

@@ -98,6 +98,7 @@ bool prompt_attention_usable(const DecoderAttention& p, int dtype);
 cudaError_t launch_prompt_attention(const DecoderAttention& p, int dtype, cudaStream_t s);
 
 // ---- sample.cu ---------------------------------------------------------------------------------------------------
+constexpr int64_t kSampleMaxVocab = 1 << 20;     // up to here a running sum is good to the step of the numbers drawn with
 struct SampleProblem {
   const void* logits;
   int64_t n, vocab;

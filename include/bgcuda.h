@@ -276,14 +276,15 @@ int bg_decoder_attention(bg_context* ctx, const bg_head_view* q, const bg_head_v
                          int64_t hkv, int64_t sq, int64_t sk, int64_t d, int dtype, const bg_attention_rules* rules,
                          const bg_head_view* out_view, bg_handle* out);
 
-/* One token per row of logits [n, vocab], as int64 [n].  Weights are e^((x - max) / temperature); a token is kept when
- * its rank (largest first, equal ones by index) is below top_k (0: all), when the weights ranked before it sum to less
- * than top_p of the first top_k (>= 1: all), and when its weight is at least min_p of the largest; the largest is always
+/* One token per row of logits [n, vocab], vocab <= 2^20, as int64 [n].  Weights are e^((x - max) / temperature); a token is
+ * kept when its rank (largest first, equal ones by index) is below top_k (0: all), when the weights ranked before it sum to
+ * less than top_p of the first top_k (>= 1: all), and when its weight is at least min_p of the largest; the largest is always
  * kept.  The result is the first kept index whose running sum in index order exceeds uniforms[row] (float32, [0, 1)) of
- * the kept sum.  Temperature 0 takes the largest, the first of equal ones.  -inf and NaN are never drawn; a row of nothing
- * else gives -1.  Per-row parameters (float32 / int32 [n]) replace the common ones when given; there a temperature that is
- * not positive is greedy, a top_k that is not positive and a top_p that is not below 1 keep all.  `probabilities`
- * (float32 [n], 0 for none) receives the chance of the token among the kept ones (1 when greedy, 0 with token -1). */
+ * the kept sum.  Running sums are off by at most vocab * 2^-47 of the largest weight below 2^18 tokens and 2^-24 of it at
+ * 2^20.  Temperature 0 takes the largest, the first of equal ones.  -inf and NaN are never drawn; a row of nothing else gives
+ * -1.  Per-row parameters (float32 / int32 [n]) replace the common ones when given; there a temperature that is not positive
+ * is greedy, a top_k that is not positive and a top_p that is not below 1 keep all.  `probabilities` (float32 [n], 0 for none)
+ * receives the chance of the token among the kept ones (1 when greedy, 0 with token -1). */
 typedef struct bg_sampling {
   double temperature, top_p, min_p;
   int64_t top_k;

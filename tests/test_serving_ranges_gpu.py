@@ -7,7 +7,7 @@ import pytest
 from browsergrad_b200 import HeadView
 from browsergrad_b200.errors import KernelError
 from tests import serving_oracle as oracle
-from tests.test_serving_gpu import DTYPES, buffers, normal, rounded, within  # noqa: F401  (buffers is a fixture)
+from tests.test_serving_gpu import DTYPES, buffers, normal, rounded, run_sample, within  # noqa: F401  (buffers is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -189,3 +189,31 @@ def test_attention_with_large_scores_stays_finite(bridge, buffers, dtype, d, sq,
     else:
         top = np.abs(rounded(v, dtype)).max()
         assert np.abs(got).max() <= top * (1 + 2.0 ** -6) and np.abs(got).max(-1).min() > 1e-3
+
+
+@pytest.mark.parametrize("vocab", [131072, 600011, 1 << 20])
+def test_sampling_reaches_a_flat_tail(bridge, buffers, vocab):
+    """One token above a tail that together has 2^-22.6 of its weight (2^-42.6 each for the largest vocabulary): the last number
+    below one falls into the tail, and the token's interval of the exact running sum lies within 2^-24 of the number."""
+    x = np.full((4, vocab), np.float32(np.log(2.0 ** -22.6 / vocab)), np.float32)
+    top = [0, 0, vocab // 2, vocab - 1]
+    x[np.arange(4), top] = 0.0
+    u = np.float32([1 - 2.0 ** -24, 1 - 2.0 ** -23, 1 - 2.0 ** -24, 2.0 ** -24])
+    got, _ = run_sample(bridge, buffers, x, u, "float32")
+    for i in range(4):
+        w = np.exp(x[i].astype(np.float64))
+        sums, at = np.cumsum(w), int(got[i])
+        # a weight is a whole number of 2^-43 of the largest or less: half a unit each, the same for equal ones
+        slack = 2.0 ** -24 * sums[-1]
+        assert 0 <= at < vocab
+        assert sums[at] - w[at] - slack <= float(u[i]) * sums[-1] <= sums[at] + slack, (i, at)
+    assert got[0] > 0
+
+
+def test_sampling_refuses_a_vocabulary_its_sums_are_too_coarse_for(bridge, buffers):
+    n = (1 << 20) + 1
+    x, u = buffers.put(np.zeros((1, n), np.float32), "float32"), buffers.put(np.zeros(1, np.float32), "float32")
+    with pytest.raises(KernelError) as e:
+        buffers.own(bridge.sample_tokens(x, u, 1, n, "float32"))
+    assert e.value.status == 2
+    assert run_sample(bridge, buffers, np.zeros((1, n - 1), np.float32), np.float32([0.5]), "float32")[0][0] == (n - 1) // 2
