@@ -158,7 +158,7 @@ cache_attention_kernel(const __grid_constant__ DecoderAttention p, int splits, i
   int len = len_in;
   if (p.lengths) {
     if (len < 0 || len > p.sk) {
-      if (tid == 0) { *p.status.host = BG_ERR_INDEX_RANGE; *p.status.device = BG_ERR_INDEX_RANGE; }
+      if (tid == 0) { *p.status.host = kStatusLength; *p.status.device = kStatusLength; }
       len = min(max(len, 0), p.sk);
     }
   }
@@ -558,7 +558,7 @@ few_rows_kernel(const __grid_constant__ DecoderAttention p, int splits, int vec,
   const int b = unit / p.hkv, hk = unit % p.hkv, n_rows = p.group * p.sq;
   const int len_in = p.lengths ? __ldg(p.lengths + b) : p.sk, start_in = p.starts ? __ldg(p.starts + b) : 0, prefix = p.prefixes ? __ldg(p.prefixes + b) : 0;
   const int len = min(max(len_in, 0), p.sk);
-  if (len != len_in && tid == 0) { *p.status.host = BG_ERR_INDEX_RANGE; *p.status.device = BG_ERR_INDEX_RANGE; }
+  if (len != len_in && tid == 0) { *p.status.host = kStatusLength; *p.status.device = kStatusLength; }
   if (tid < 4) {
     int hi = 0, doc = -1;
     long long pos = 0;

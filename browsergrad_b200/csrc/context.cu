@@ -448,7 +448,7 @@ int bg_selftest_wait_timeout(bg_context* ctx, int64_t limit_cycles) {
   if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "selftest_wait_timeout");
   const int st = take_device_status(ctx);
-  if (st != 0) return fail(ctx, st, device_status_message(st));
+  if (st != 0) return fail_device_status(ctx, st, "");
   return BG_OK;
 }
 
@@ -480,7 +480,7 @@ int bg_materialize(bg_context* ctx, bg_handle h, void* out, size_t nbytes) {
   if (rc == BG_OK && ctx->status_pending) {
     // d2h synchronised the stream: the status copy behind the producing plan has landed
     const int st = take_device_status(ctx);
-    if (st != 0) return fail(ctx, st, device_status_message(st) + " (in the plan that produced this buffer or an earlier one)");
+    if (st != 0) return fail_device_status(ctx, st, " (in the work that produced this buffer, or earlier)");
   }
   return rc;
 }
@@ -544,7 +544,7 @@ int bg_flush_profiles(bg_context* ctx, bg_profile_entry* out, int capacity, int*
   if (e != cudaSuccess) return cuda_fail(ctx, e, "flush_profiles synchronize");
   if (ctx->status_pending) {
     const int st = take_device_status(ctx);
-    if (st != 0) return fail(ctx, st, device_status_message(st) + " (in an earlier plan)");
+    if (st != 0) return fail_device_status(ctx, st, kInEarlierWork);
   }
   for (auto& pe : ctx->pending_events) {
     float ms = 0.f;

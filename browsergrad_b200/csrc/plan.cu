@@ -15,6 +15,7 @@
 //   7. units are scheduled topologically, intermediates are allocated stream-ordered at first
 //      use and freed after their last reader.
 #include "runtime.h"
+#include "serving.h"
 
 #include <string.h>
 
@@ -3541,10 +3542,16 @@ int take_early_status(bg_context* ctx) {
   return take_device_status(ctx);
 }
 
-std::string device_status_message(int status_rc) {
-  return status_rc == BG_ERR_INDEX_RANGE ? "run_tensor_plan: gather / scatter / cross_entropy index outside its axis, scatter indices naming one destination twice, or a length, count or cache row outside its buffer"
-         : status_rc == BG_ERR_DEVICE_TIMEOUT ? "run_tensor_plan: a device-side wait of a tensor-core kernel gave up (status 6)"
-                                              : "run_tensor_plan: device-side status " + std::to_string(status_rc);
+int fail_device_status(bg_context* ctx, int status, const char* where) {
+  const int code = status & 0xff;
+  std::string m;
+  if (status == kStatusAppend) m = "rotary_append: a count or a cache row outside its buffer";
+  else if (status == kStatusLength) m = "decoder_attention: a length outside the cache";
+  else if (status == kStatusPromptWait) m = "decoder_attention: a device-side wait of the prompt kernel gave up (status 6)";
+  else if (code == BG_ERR_INDEX_RANGE) m = "run_tensor_plan: gather / scatter / cross_entropy index outside its axis, or scatter indices naming one destination twice";
+  else if (code == BG_ERR_DEVICE_TIMEOUT) m = "run_tensor_plan: a device-side wait of a tensor-core kernel gave up (status 6)";
+  else m = "run_tensor_plan: device-side status " + std::to_string(status);
+  return fail(ctx, code, m + where);
 }
 
 int run_plan(bg_context* ctx, const bg_plan* plan, const bg_plan_input* inputs, int n_inputs, void* out_host,
@@ -3553,7 +3560,7 @@ int run_plan(bg_context* ctx, const bg_plan* plan, const bg_plan_input* inputs, 
   if (n_inputs > 0 && !inputs) return fail(ctx, BG_ERR_INVALID, "run_tensor_plan: null inputs");
   cudaSetDevice(ctx->device);
   // a device-side wait that gave up in an earlier plan whose root stayed on the device is reported here at the latest
-  if (const int st = take_early_status(ctx)) return fail(ctx, st, device_status_message(st) + " (in an earlier plan)");
+  if (const int st = take_early_status(ctx)) return fail_device_status(ctx, st, kInEarlierWork);
   uint64_t h = 1469598103934665603ull;
   h = fnv1a(plan->steps, sizeof(bg_plan_step) * (size_t)plan->n_steps, h);
   if (plan->n_ext > 0) h = fnv1a(plan->ext, sizeof(int32_t) * (size_t)plan->n_ext, h);
@@ -3676,7 +3683,7 @@ int run_plan(bg_context* ctx, const bg_plan* plan, const bg_plan_input* inputs, 
   }
   if (status_rc) {
     cleanup(false);
-    return fail(ctx, status_rc, device_status_message(status_rc));
+    return fail_device_status(ctx, status_rc, "");
   }
   if (out_host) {
     int rc = d2h(ctx, out_host, run.ptr[cp->root_slot], (size_t)cp->root_bytes);
@@ -3684,7 +3691,7 @@ int run_plan(bg_context* ctx, const bg_plan* plan, const bg_plan_input* inputs, 
     if (rc == BG_OK && ctx->status_pending) {
       // the copy synchronised the stream: what earlier work refused on the device is known now
       const int st = take_device_status(ctx);
-      if (st != 0) return fail(ctx, st, device_status_message(st) + " (in an earlier plan)");
+      if (st != 0) return fail_device_status(ctx, st, kInEarlierWork);
     }
     return rc;
   }

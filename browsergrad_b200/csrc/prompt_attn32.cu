@@ -447,7 +447,7 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
-    if (threadIdx.x == 0) { *a.status.host = BG_ERR_DEVICE_TIMEOUT; *a.status.device = BG_ERR_DEVICE_TIMEOUT; }
+    if (threadIdx.x == 0) { *a.status.host = kStatusPromptWait; *a.status.device = kStatusPromptWait; }
     const long long t0 = clock64();
     while (clock64() - t0 < 200000) {}
     __syncthreads();

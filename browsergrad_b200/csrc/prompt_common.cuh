@@ -46,7 +46,7 @@ struct Sequence {
 };
 __device__ __forceinline__ Sequence sequence_of(const DecoderAttention& a, int b) {
   const int n = a.lengths ? __ldg(a.lengths + b) : a.sk, st = a.starts ? __ldg(a.starts + b) : 0, pre = a.prefixes ? __ldg(a.prefixes + b) : 0;
-  if ((n < 0 || n > a.sk) && threadIdx.x == 0) { *a.status.host = BG_ERR_INDEX_RANGE; *a.status.device = BG_ERR_INDEX_RANGE; }
+  if ((n < 0 || n > a.sk) && threadIdx.x == 0) { *a.status.host = kStatusLength; *a.status.device = kStatusLength; }
   const int len = min(max(n, 0), a.sk);
   return Sequence{len, pre, a.starts ? (long long)st : (long long)len - a.sq};
 }

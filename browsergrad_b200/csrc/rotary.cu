@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
   if (p.counts) {
     count = p.counts[batch];
     if (count < 0 || count > p.s) {
-      if (threadIdx.x == 0) { *p.status.host = BG_ERR_INDEX_RANGE; *p.status.device = BG_ERR_INDEX_RANGE; }
+      if (threadIdx.x == 0) { *p.status.host = kStatusAppend; *p.status.device = kStatusAppend; }
       count = count < 0 ? 0 : p.s;
     }
   }
@@ -116,8 +116,8 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
       keep = s0 + tok < count;
       row_out += first;
       if (keep && (row_out < 0 || row_out >= p.capacity)) {
-        *p.status.host = BG_ERR_INDEX_RANGE;
-        *p.status.device = BG_ERR_INDEX_RANGE;
+        *p.status.host = kStatusAppend;
+        *p.status.device = kStatusAppend;
         keep = false;
       }
     }

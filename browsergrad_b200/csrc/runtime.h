@@ -111,7 +111,9 @@ int take_device_status(bg_context* ctx);
 // The same ahead of new work, without waiting as long as nothing has been reported: 0, or the status of earlier work, whose
 // stream has then been synchronised.
 int take_early_status(bg_context* ctx);
-std::string device_status_message(int status_rc);
+// Fails with what a status word says: its low byte is the bg_status, the rest who reported it (kStatus... in serving.h, else a plan).
+int fail_device_status(bg_context* ctx, int status, const char* where);
+constexpr const char* kInEarlierWork = " (in an earlier plan or call)";
 int run_plan(bg_context* ctx, const bg_plan* plan, const bg_plan_input* inputs, int n_inputs, void* out_host,
              size_t out_nbytes, bg_handle* out_handle);
 

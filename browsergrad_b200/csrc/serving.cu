@@ -32,7 +32,7 @@ int begin(const Call& c) {
   cudaError_t e = cudaStreamIsCapturing(c.ctx->stream, &cap);
   if (e != cudaSuccess) return cuda_fail(c.ctx, e, c.op);
   if (cap != cudaStreamCaptureStatusNone) return c.error(BG_ERR_UNSUPPORTED, "the bridge's stream is being captured into a graph");
-  if (const int st = take_early_status(c.ctx)) return fail(c.ctx, st, device_status_message(st) + " (in an earlier plan)");
+  if (const int st = take_early_status(c.ctx)) return fail_device_status(c.ctx, st, kInEarlierWork);
   return BG_OK;
 }
 

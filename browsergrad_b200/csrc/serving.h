@@ -16,6 +16,10 @@ struct StatusWords {
   int* device;
   int* host;
 };
+// What they report there: a bg_status in the low byte, the operator above it.
+constexpr int kStatusAppend = BG_ERR_INDEX_RANGE | 1 << 8;
+constexpr int kStatusLength = BG_ERR_INDEX_RANGE | 2 << 8;
+constexpr int kStatusPromptWait = BG_ERR_DEVICE_TIMEOUT | 3 << 8;
 
 // Raises a kernel's limit of dynamic shared memory where it is below `bytes`, which is remembered (the call costs about a
 // microsecond).  The limit belongs to the kernel on its device and is shared by all threads and contexts: it is never

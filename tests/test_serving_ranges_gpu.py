@@ -4,7 +4,7 @@ from concurrent.futures import ThreadPoolExecutor
 import numpy as np
 import pytest
 
-from browsergrad_b200 import HeadView
+from browsergrad_b200 import HeadView, RotarySpec
 from browsergrad_b200.errors import KernelError
 from tests import serving_oracle as oracle
 from tests.test_serving_gpu import DTYPES, buffers, normal, rounded, run_sample, within  # noqa: F401  (buffers is a fixture)
@@ -217,3 +217,18 @@ def test_sampling_refuses_a_vocabulary_its_sums_are_too_coarse_for(bridge, buffe
         buffers.own(bridge.sample_tokens(x, u, 1, n, "float32"))
     assert e.value.status == 2
     assert run_sample(bridge, buffers, np.zeros((1, n - 1), np.float32), np.float32([0.5]), "float32")[0][0] == (n - 1) // 2
+
+
+@pytest.mark.parametrize("sq", [1, 64])
+def test_a_device_side_refusal_names_its_operator(bridge, buffers, sq):
+    x = buffers.put(normal(1, 1, 1, sq, 64), "bfloat16")
+    caches = [buffers.put(normal(2, 1, 1, 80, 64), "bfloat16") for _ in range(2)]
+    bad = buffers.put(np.array([81]), "int32")
+    out = buffers.own(bridge.decoder_attention(x, *caches, 1, 1, 1, sq, 80, 64, "bfloat16", lengths=bad))
+    with pytest.raises(KernelError, match="decoder_attention: a length outside the cache") as e:
+        bridge.materialize(out, (1, 1, sq, 64), "bfloat16")
+    assert e.value.status == 7
+    out = buffers.own(bridge.rotary_append(x, x, x, *caches, RotarySpec(64), 1, 1, 1, sq, 80, 64, "bfloat16", starts=bad))
+    with pytest.raises(KernelError, match="rotary_append: a count or a cache row outside its buffer") as e:
+        bridge.synchronize()
+    assert e.value.status == 7
