@@ -219,8 +219,10 @@ int bg_flash_attention(bg_context* ctx, bg_handle q, bg_handle k, bg_handle v, b
  *    Results are written into `out_view` / `out_handle` when one is given (the caller's buffer; it must be none of the
  *    call's other operands), else into a buffer minted for them.  Index buffers are int32.  A call into a stream that is
  *    being captured into a graph is refused (BG_ERR_UNSUPPORTED).  Values only the device sees (lengths, counts, cache
- *    rows) are range-checked there: one outside its range is treated as the nearest legal one, nothing outside a buffer
- *    is touched, and the next call that synchronises or starts other work returns BG_ERR_INDEX_RANGE. --------------- */
+ *    rows) are range-checked there: a length or count outside its range is cut to it, a new row outside its cache is
+ *    dropped, nothing outside a buffer is touched.  The next call that synchronises returns BG_ERR_INDEX_RANGE, or an
+ *    earlier one that starts other work and finds the report there; either has waited for all work before it and returns
+ *    the status once for all of it. ---------------------------------------------------------------------------- */
 
 /* Where the heads of a tensor lie in a buffer: head h of row s of batch b is the d consecutive values from element
  * offset + b * stride[0] + s * stride[1] + h * stride[2].  Any order of the axes, rows of a packed projection, a range of
@@ -235,7 +237,8 @@ typedef enum bg_rotary_scaling { BG_ROTARY_PLAIN = 0, BG_ROTARY_LINEAR = 1, BG_R
 /* The first `dim` values of a head (even, <= 256) are pairs: (2j, 2j + 1) when interleaved, else (j, j + dim / 2); pair j
  * of a row at position t is turned by t * f_j, f_j = base^(-2j / dim), and multiplied by `magnitude`; the values behind
  * `dim` are copied.  LINEAR: f_j / factor.  RAMP: f_j * (g + (1 - g) / factor) with g = clamp((original_length * f_j /
- * 2 pi - low) / (high - low), 0, 1): pairs that turn often within the original length keep their frequency. */
+ * 2 pi - low) / (high - low), 0, 1): pairs that turn often within the original length keep their frequency.  The angle is a
+ * 64-bit product (off by 2^-52 of itself), its sine and cosine and the rotation are 32-bit. */
 typedef struct bg_rotary_spec {
   int32_t dim, interleaved, scaling, reserved;
   double base, factor, low, high, original_length, magnitude;
