@@ -4,14 +4,17 @@
 // The structure is that of the fp32 attention of a plan (attn_tf32_row.cu): one CTA owns 128 query rows of a head and
 // walks tiles of 64 keys; Q, K and V arrive as the caller's rows (TMA), converter warps round them to hi = tf32(x) in place
 // and write lo = x - hi; S = lo.hi + hi.lo + hi.hi in a double-buffered accumulator; one thread per query row takes the
-// maximum, the exponentials and the sum without exchange and leaves P as hi / lo planes in tensor memory; O is folded into
-// registers every eight tiles, because the tensor core adds with truncation.
+// maximum, the exponentials and the sum without exchange and leaves P as hi / lo planes in tensor memory; P V of a key tile
+// starts from zero in one of two accumulators and is added to O in registers while the next tile's runs, because the tensor core
+// adds with truncation: eight tiles added there, three products each, left a bias of 5 * 10^-6 of the result, this way 3 * 10^-7.
 //   warp 0 producer, warp 1 issues the products, warps 2 and 3 convert V, warps 4-7 softmax, warps 8-11 convert Q and K
-// What differs is what the rules ask: shared key heads, a visible range and a document per row instead of a mask tensor,
-// cap and bias, and value rows behind the sequence's length become zeros as they are converted.  The cap is the library's
-// tanhf: its error is scaled by the cap into the exponent, and fp32 results are held to some 10^-6.
-// Measured: 8 x 12 heads of 1024 tokens of 64, biased, 119 us (29 us as three tf32 products at half the bf16 rate); the tensor
-// pipe is 25 % busy: products and softmax of the one query tile an SM holds take turns.
+// What differs is that addition (there O is folded every eight tiles) and what the rules ask: shared key heads, a visible range
+// and a document per row instead of a mask tensor, cap and bias, and value rows behind the sequence's length become zeros as
+// they are converted.  The cap is the library's tanhf: its error is scaled by the cap into the exponent, and fp32 results are
+// held to some 10^-6.
+// Rounded to fewer bits than 32: nothing is left out but the products lo.lo and the bits of lo that tf32 drops, 2^-21 of a term.
+// Measured: 8 x 12 heads of 1024 tokens of 64, biased, 137 us, causal without bias 132 (the eight-tile sums 141 and 133; 29 us as
+// three tf32 products at half the bf16 rate); products and softmax of the one query tile an SM holds take turns.
 // No cluster multicast; every wait is clock-bounded.
 #include "serving.h"
 
@@ -38,21 +41,9 @@ constexpr int kQBytes = 4 * kRows * 128, kKBytes = 4 * kKeys * 128, kVBytes = 4 
 constexpr int kSmem = kQBytes + kStagesK * kKBytes + kStagesV * kVBytes;
 constexpr int kLaunchRegs = 168, kLightRegs = 72, kSoftmaxRegs = 248;
 static_assert(256 * kLightRegs + 128 * kSoftmaxRegs <= kLaunchRegs * kThreads, "setmaxnreg requests exceed the CTA's registers");
-constexpr int kColS = 0, kColP = 128, kColO = 384;      // 2 x 64, 2 x (hi 64 | lo 64), 64
-constexpr int kChunkTiles = 8;                          // key tiles summed in tensor memory before O is folded into registers
+constexpr int kColS = 0, kColP = 128, kColO = 384;      // 2 x 64, 2 x (hi 64 | lo 64), 2 x 64
 constexpr float kLazyLog2 = 8.0f, kLog2e = 1.4426950408889634f;
 constexpr uint32_t kVHalf = kKeys * 128;
-
-__device__ __noinline__ void rescale_row(uint32_t t_o, float alpha) {
-#pragma unroll 1
-  for (int half = 0; half < 2; ++half) {
-    uint32_t r[32];
-    tmem_ld32(t_o + (uint32_t)(half * 32), r);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-    tmem_st32(t_o + (uint32_t)(half * 32), r);
-  }
-}
 
 __device__ __forceinline__ void umma_ts_tf32(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -213,15 +204,14 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         if (!wait_all(&p_full[buf], (uint32_t)(t >> 1) & 1u)) return false;
         if (!wait_all(&v_full[s], (uint32_t)(t / kStagesV) & 1u)) return false;
         tc_fence_after();
-        const uint32_t v_addr = smem_u32(sV + s * kVBytes), t_p = tmem_base + (uint32_t)(kColP + buf * 2 * kKeys), d_o = tmem_base + (uint32_t)kColO;
-        const uint32_t fresh = (t % kChunkTiles) == 0 ? 0u : 1u;       // a chunk's first product starts a new accumulator
+        const uint32_t v_addr = smem_u32(sV + s * kVBytes), t_p = tmem_base + (uint32_t)(kColP + buf * 2 * kKeys), d_o = tmem_base + (uint32_t)(kColO + buf * kDim);
         if (elect_one()) {
 #pragma unroll
           for (int pass = 0; pass < 3; ++pass) {
             const uint32_t pa = t_p + (pass == 0 ? (uint32_t)kKeys : 0u), va = v_addr + (pass == 1 ? 2 * kVHalf : 0);
 #pragma unroll
             for (int g = 0; g < 8; ++g)      // groups of 8 keys
-              umma_ts_tf32(d_o, pa + (uint32_t)(g * 8), make_v_rows_desc(va + (uint32_t)(g * 1024)), idesc_pv, (pass | g) ? 1u : fresh);
+              umma_ts_tf32(d_o, pa + (uint32_t)(g * 8), make_v_rows_desc(va + (uint32_t)(g * 1024)), idesc_pv, (pass | g) ? 1u : 0u);
           }
           umma_commit(&pv_full[buf]);
           umma_commit(&v_empty[s]);
@@ -277,7 +267,7 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     const int quarter = warp & 3, row = q0 + quarter * 32 + lane;
     const bool row_ok = row < a.sq;
     const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
-    float o[kDim];                                   // the chunks folded so far, relative to m_ref
+    float o[kDim];                                   // the key tiles added so far, relative to m_ref
 #pragma unroll
     for (int d = 0; d < kDim; ++d) o[d] = 0.f;
     float m_ref = -CUDART_INF_F, l = 0.f;            // in powers of two
@@ -291,11 +281,14 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     const float slope = BIAS && a.slopes ? a.slopes[h] * kLog2e : 0.f;
     const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, to_cap = CAP ? a.scale / a.cap : 0.f;
     constexpr bool FOLD = !CAP && !BIAS;             // the scale is applied in the exponent (it is positive then)
-    const uint32_t t_o = tmem_base + (uint32_t)kColO + lane_sel;
     bool ok = true;
     int t = 0;
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
-    auto fold_chunk = [&]() {
+    // Adds P V of tile u, once it has completed, and takes the sum to the reference that tile u + 1 set.
+    auto add_tile = [&](int u, float alpha) -> bool {
+      if (!wait_warp(&pv_full[u & 1], (uint32_t)(u >> 1) & 1u)) return false;
+      tc_fence_after();
+      const uint32_t t_o = tmem_base + (uint32_t)(kColO + (u & 1) * kDim) + lane_sel;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t r[32];
@@ -303,6 +296,12 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[half * 32 + i] = __fadd_rn(o[half * 32 + i], __uint_as_float(r[i]));
       }
+      if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll
+        for (int d = 0; d < kDim; ++d) o[d] *= alpha;
+      }
+      tc_fence_before();
+      return true;
     };
     for (int j = 0; j < n_kv && ok; ++j) {
       if (!s_need[j]) continue;
@@ -364,37 +363,15 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         if (FOLD) mt *= to_log2;
       }
       const bool coarse = FOLD && fabsf(mt) >= kCoarse && mt != -CUDART_INF_F;
-      // Chunk boundary: O is folded into registers before this tile's P V starts a fresh accumulator.
-      bool o_quiet = t == 0;
-      if (t > 0 && (t % kChunkTiles) == 0) {
-        ok = wait_warp(&pv_full[(t - 1) & 1], (uint32_t)((t - 1) >> 1) & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        fold_chunk();
-        o_quiet = true;
-      }
       const bool raise = m_ref != -CUDART_INF_F && mt - m_ref > kLazyLog2;
       float unit = to_log2;                           // FOLD: what the scores are still to be multiplied by
-      if (__any_sync(0xffffffffu, raise || coarse)) {
-        if (FOLD && __any_sync(0xffffffffu, coarse)) {
+      if (FOLD && __any_sync(0xffffffffu, coarse)) {
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i) x[i] *= to_log2;
-          unit = 1.0f;
-        }
-        const float alpha = raise ? ex2_approx(m_ref - mt) : 1.0f;
-        if ((t % kChunkTiles) != 0) {                // the current chunk holds products: they must be complete
-          if (!o_quiet) {
-            ok = wait_warp(&pv_full[(t - 1) & 1], (uint32_t)((t - 1) >> 1) & 1u);
-            if (!ok) break;
-            tc_fence_after();
-          }
-          rescale_row(t_o, alpha);
-          tc_fence_before();
-        }
-#pragma unroll
-        for (int d = 0; d < kDim; ++d) o[d] *= alpha;
-        if (raise) { l *= alpha; m_ref = mt; }
+        for (int i = 0; i < kKeys; ++i) x[i] *= to_log2;
+        unit = 1.0f;
       }
+      const float alpha = raise ? ex2_approx(m_ref - mt) : 1.0f;
+      if (raise) { l *= alpha; m_ref = mt; }
       if (m_ref == -CUDART_INF_F) m_ref = mt;
       const float off = m_ref == -CUDART_INF_F ? 0.f : -m_ref;
       {
@@ -406,11 +383,8 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         }
         l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
       }
-      if (t >= 2) {                                   // this P buffer was read by the P V of tile t - 2
-        ok = wait_warp(&pv_full[buf], (uint32_t)((t - 2) >> 1) & 1u);
-        if (!ok) break;
-      }
       {
+        // (P V of tile t - 2, which read this buffer, has been added)
         const uint32_t t_p = tmem_base + (uint32_t)(kColP + buf * 2 * kKeys) + lane_sel;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -429,12 +403,11 @@ prompt_attention32_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[buf]);
+      if (t > 0) ok = add_tile(t - 1, alpha);         // while P V of this tile runs
       ++t;
     }
-    if (ok && t > 0) ok = wait_warp(&pv_full[(t - 1) & 1], (uint32_t)((t - 1) >> 1) & 1u);
+    if (ok && t > 0) ok = add_tile(t - 1, 1.0f);
     if (ok) {
-      tc_fence_after();
-      if (t > 0) fold_chunk();                        // the last chunk (warp-wide loads; only the stores are per row)
       if (row_ok) {
         const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);      // a row without keys is zero; NaN stays NaN
         float* out = reinterpret_cast<float*>(const_cast<void*>(a.out.ptr)) + b * a.out.sb + (long long)h * a.out.sh + (long long)row * a.out.sr;

@@ -232,3 +232,24 @@ def test_a_device_side_refusal_names_its_operator(bridge, buffers, sq):
     with pytest.raises(KernelError, match="rotary_append: a count or a cache row outside its buffer") as e:
         bridge.synchronize()
     assert e.value.status == 7
+
+
+@pytest.mark.parametrize("d", [32, 64])
+@pytest.mark.parametrize("sq,sk", [(64, 512), (128, 448), (200, 512)])
+def test_attention_of_float32_prompts_adds_without_a_bias(bridge, buffers, d, sq, sk):
+    """Nearly equal scores over values of one sign: the result is a mean, to which every key adds.  An error e_j in the exponent
+    of probability p_j moves it by p_j e_j (v_j - mean); e_j: the dot product as in attention(), scaling and exponential 2^-21.
+    The rest is relative to the mean: the split of probabilities and of values drops 2^-21 each; the tensor core adds with
+    truncation, a step of 2^-23 for each of a tile's 8 products of the upper parts and two more for the small ones; the tiles are
+    added in 32 bits, half a step each, the probabilities by 18 such additions in a tile and one for each tile, and the division
+    and its product are two halves more."""
+    q, k = 0.05 * normal(4, 2, 2, sq, d), normal(6, 2, 2, sk, d)
+    v = 3.0 + np.clip(normal(5, 2, 2, sk, d), -3, 3) / 4
+    got = attend(bridge, buffers, "float32", q, k, v, causal=False)
+    q, k, v = (x.astype(np.float64) for x in (q, k, v))
+    p = np.exp(q @ k.swapaxes(-1, -2) / np.sqrt(d))
+    p /= p.sum(-1, keepdims=True)
+    want = p @ v
+    p = p * ((d + 16) * 2.0 ** -23 * (np.abs(q) @ np.abs(k).swapaxes(-1, -2)) / np.sqrt(d) + 2.0 ** -21)
+    err = p @ np.abs(v - 3.0) + p.sum(-1, keepdims=True) * np.abs(want - 3.0) + want * (2 * 2.0 ** -21 + 10 * 2.0 ** -23 + (2 * (sk // 64) + 18 + 2) * 2.0 ** -24)
+    within(got, want, err)
