@@ -48,6 +48,12 @@ using attn::tma_load_4d;
 constexpr int kRows = 128, kKeys = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyLog2 = 8.0f;
+// Key tiles that are added in tensor memory before O goes to a sum in memory (LONG: caches that have more).  The tensor core adds
+// with truncation, which makes a result smaller by some 6 * 10^-8 for each addition, eight a tile: 3 * 10^-5 after 64 tiles, but
+// 6 * 10^-4 after 131072 keys, more than the half step of float16.  64 rows of 8 heads of 128 over 131072 keys: 2144 us without
+// the sums in memory, 2212 with them; their code alone would cost plain prompts of heads of 64 a tenth (394 -> 430 us), hence
+// kernels of their own.
+constexpr int kFoldTiles = 64;
 // float16 probabilities lie up to 2^7 above the reference, 2^15 with the lazy maximum, where the type still has room: against
 // the maximum itself they would vanish below 2^-25 of it while their sum still counted them.  It cancels in the division.
 constexpr float kRoomF16 = 7.0f;
@@ -132,6 +138,25 @@ __device__ __noinline__ void rescale_row(uint32_t t_o, float alpha) {
   }
 }
 
+// Adds a row's O to its sum in memory, [D] values and their reference, 128 rows side by side: O goes on from zero.
+template <int D>
+__device__ __noinline__ void fold_row(uint32_t t_o, float* sum, float m_ref, bool first) {
+  const float from = first ? -CUDART_INF_F : sum[D * kRows];
+  const float f = from == -CUDART_INF_F ? 0.f : ex2_approx(from - m_ref);
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t r[32];
+    tmem_ld32(t_o + (uint32_t)(c * 32), r);
+    float* p = sum + c * 32 * kRows;
+    float before[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) before[i] = first ? 0.f : p[i * kRows];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) p[i * kRows] = fmaf(before[i], f, __uint_as_float(r[i]));
+  }
+  sum[D * kRows] = m_ref;
+}
+
 // Caps the scores of a row's key tile in tensor memory, some of them beyond the cap.  Each value takes the form that is accurate
 // relative to it; within the cap that is the polynomial with the very operations of the main path, so that a score's bits do
 // not depend on its neighbours.  Beyond it 1 - 2 / (1 + e^2x) is off by at most 2^-21, of a value above 0.76.  Out of line and
@@ -163,7 +188,7 @@ __device__ __noinline__ void cap_mixed_row(uint32_t t_s, float to_cap, float to_
   }
 }
 
-template <bool BF16, int D, int NT, bool CAP, bool BIAS>
+template <bool BF16, int D, int NT, bool CAP, bool BIAS, bool LONG>
 __global__ void __launch_bounds__(Cfg<D, NT>::Threads, Cfg<D, NT>::PerSm)
 prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const __grid_constant__ PromptParams pp) {
@@ -303,7 +328,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             // rows of V are the K index: 16 of them are 2048 bytes; the second 64 values of a row lie a box further on
             uint64_t db = make_mnmajor_sw128_desc(v_addr + (uint32_t)(k * 2048));
             if (C::Boxes == 2) db = (db & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(C::BoxBytes >> 4) << 16);
-            umma_ts_f16(d_o, d_p + (uint32_t)(k * 8), db, idesc_pv, n > 0 || k > 0 ? 1u : 0u);
+            umma_ts_f16(d_o, d_p + (uint32_t)(k * 8), db, idesc_pv, (LONG ? n % kFoldTiles != 0 : n > 0) || k > 0 ? 1u : 0u);
           }
           umma_commit(&pv_full[g]);
         }
@@ -482,7 +507,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         bool pv_done = t == 0 || C::Alias;
         const bool raise = m_ref != -CUDART_INF_F && mt - m_ref > kLazyLog2;
         float unit = to_log2;                               // FOLD: what the scores are still to be multiplied by
-        if (FOLD ? __any_sync(0xffffffffu, raise || coarse) : __any_sync(0xffffffffu, raise)) {
+        const bool fold = LONG && t % kFoldTiles == 0 && t > 0;
+        if (FOLD ? __any_sync(0xffffffffu, raise || coarse || fold) : __any_sync(0xffffffffu, raise || fold)) {
           if (FOLD && __any_sync(0xffffffffu, coarse)) {
 #pragma unroll
             for (int i = 0; i < kKeys; ++i) x[i] *= to_log2;
@@ -495,7 +521,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             tc_fence_after();
           }
           const float alpha = raise ? ex2_approx(m_ref - mt) : 1.0f;
-          rescale_row<D>(t_o, alpha);
+          if (fold) fold_row<D>(t_o, a.sums + ((size_t)blockIdx.x * NT + g) * ((D + 1) * kRows) + r_in_tile, m_ref, t == kFoldTiles);
+          else rescale_row<D>(t_o, alpha);
           if (raise) { l *= alpha; m_ref = mt; }
         }
         if (m_ref == -CUDART_INF_F) m_ref = mt;
@@ -559,11 +586,16 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       if (ok) {
         tc_fence_after();
         const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);      // a row without keys is zero; NaN stays NaN
+        const float* sum = LONG && t > kFoldTiles ? a.sums + ((size_t)blockIdx.x * NT + g) * ((D + 1) * kRows) + r_in_tile : nullptr;
+        const float from = sum ? sum[D * kRows] : -CUDART_INF_F, f = from == -CUDART_INF_F ? 0.f : ex2_approx(from - m_ref);
         uint16_t* out = reinterpret_cast<uint16_t*>(const_cast<void*>(a.out.ptr)) + b * a.out.sb + (long long)h * a.out.sh + (long long)(row_ok ? row : 0) * a.out.sr;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t r[32];
           if (t > 0) tmem_ld32(t_o + (uint32_t)(c * 32), r);
+          if (LONG && sum)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(sum[(c * 32 + i) * kRows], f, __uint_as_float(r[i])));
           if (row_ok) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
@@ -596,9 +628,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 template <int D, int NT>
 size_t smem_bytes(int sk) { return (size_t)Cfg<D, NT>::Smem + 1024 + 256 + NT * (size_t)((sk + kKeys - 1) / kKeys); }
 
-template <bool BF16, int D, int NT, bool CAP, bool BIAS>
+template <bool BF16, int D, int NT, bool CAP, bool BIAS, bool LONG>
 cudaError_t launch_kernel(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
-  auto kern = prompt_attention_kernel<BF16, D, NT, CAP, BIAS>;
+  auto kern = prompt_attention_kernel<BF16, D, NT, CAP, BIAS, LONG>;
   static const int regs = [&] {
     cudaFuncAttributes fa;
     return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
@@ -614,12 +646,27 @@ cudaError_t launch_kernel(const PromptParams& p, const CUtensorMap& q, const CUt
   return cudaGetLastError();
 }
 
+template <bool BF16, int D, int NT, bool CAP, bool BIAS>
+cudaError_t launch_length(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
+  return p.a.sums ? launch_kernel<BF16, D, NT, CAP, BIAS, true>(p, q, k, v, s) : launch_kernel<BF16, D, NT, CAP, BIAS, false>(p, q, k, v, s);
+}
+
 template <bool BF16, int D, int NT>
 cudaError_t launch_rules(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
   // a scale that is not positive cannot be taken out of the row maximum: such scores are scaled like biased ones
   const bool bias = p.a.slopes || !(p.a.scale > 0.f), cap = p.a.cap > 0.f;
-  if (cap) return bias ? launch_kernel<BF16, D, NT, true, true>(p, q, k, v, s) : launch_kernel<BF16, D, NT, true, false>(p, q, k, v, s);
-  return bias ? launch_kernel<BF16, D, NT, false, true>(p, q, k, v, s) : launch_kernel<BF16, D, NT, false, false>(p, q, k, v, s);
+  if (cap) return bias ? launch_length<BF16, D, NT, true, true>(p, q, k, v, s) : launch_length<BF16, D, NT, true, false>(p, q, k, v, s);
+  return bias ? launch_length<BF16, D, NT, false, true>(p, q, k, v, s) : launch_length<BF16, D, NT, false, false>(p, q, k, v, s);
+}
+
+// Query tiles of a CTA.
+int query_tiles(const DecoderAttention& p) {
+  if (p.d > 64) return 2;
+  // One query tile a CTA and two CTAs an SM where there is little work behind a CTA's start, which the other then covers:
+  // 32 x 128 tokens 18 us against 24, 16 x 512 33 against 35 (capped 45 against 49), packed documents of 400 in 4 x 2048
+  // 46 against 49; from 2048 keys on two tiles that share their keys and take turns win (capped 99.5 us against 101.5,
+  // 16 heads of 4096 keys 683 against 773).
+  return p.documents || p.sk <= 1024 ? 1 : 2;
 }
 
 }  // namespace
@@ -635,6 +682,12 @@ bool prompt_attention_usable(const DecoderAttention& p, int dtype) {
   return view_fits(p.q, dtype, p.b, p.sq, p.hq) && view_fits(p.k, dtype, p.b, p.sk, p.hkv) && view_fits(p.v, dtype, p.b, p.sk, p.hkv) && view_fits(p.out, dtype, p.b, p.sq, p.hq);
 }
 
+int64_t prompt_attention_scratch(const DecoderAttention& p, int dtype) {
+  if (dtype == BG_F32 || p.sk <= kFoldTiles * kKeys) return 0;
+  const int64_t nt = query_tiles(p), ctas = (((p.sq + kRows - 1) / kRows + nt - 1) / nt) * (int64_t)p.b * p.hq;
+  return ctas * nt * ((p.d > 64 ? 128 : 64) + 1) * kRows * (int64_t)sizeof(float);
+}
+
 cudaError_t launch_prompt_attention(const DecoderAttention& p, int dtype, cudaStream_t s) {
   if (dtype == BG_F32) return launch_prompt_attention32(p, s);
   CUtensorMap q, k, v;
@@ -647,11 +700,7 @@ cudaError_t launch_prompt_attention(const DecoderAttention& p, int dtype, cudaSt
   pp.idesc_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
   pp.idesc_pv = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)((wide ? 128 : 64) >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);   // V is MN-major
   if (wide) return bf ? launch_rules<true, 128, 2>(pp, q, k, v, s) : launch_rules<false, 128, 2>(pp, q, k, v, s);
-  // One query tile a CTA and two CTAs an SM where there is little work behind a CTA's start, which the other then covers:
-  // 32 x 128 tokens 18 us against 24, 16 x 512 33 against 35 (capped 45 against 49), packed documents of 400 in 4 x 2048
-  // 46 against 49; from 2048 keys on two tiles that share their keys and take turns win (capped 99.5 us against 101.5,
-  // 16 heads of 4096 keys 683 against 773).
-  if (p.documents || p.sk <= 1024) return bf ? launch_rules<true, 64, 1>(pp, q, k, v, s) : launch_rules<false, 64, 1>(pp, q, k, v, s);
+  if (query_tiles(p) == 1) return bf ? launch_rules<true, 64, 1>(pp, q, k, v, s) : launch_rules<false, 64, 1>(pp, q, k, v, s);
   return bf ? launch_rules<true, 64, 2>(pp, q, k, v, s) : launch_rules<false, 64, 2>(pp, q, k, v, s);
 }
 

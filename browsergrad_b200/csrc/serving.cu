@@ -354,6 +354,10 @@ int decoder_attention(const Call& c, const bg_head_view* q, const bg_head_view* 
       if (int rc = launch(c, "doc_ranges", 1, [&] { return launch_doc_ranges(documents, p.b, p.sk, reinterpret_cast<int2*>(ranges.p), c.ctx->stream); })) return rc;
     }
     if (prompt_attention_usable(p, dtype)) {
+      if (const int64_t bytes = prompt_attention_scratch(p, dtype)) {
+        if (int rc = partials.get(bytes)) return rc;
+        p.sums = reinterpret_cast<float*>(partials.p);
+      }
       if (int rc = launch(c, std::string("prompt_attention[") + dtype_name(dtype) + "]", 1, [&] { return launch_prompt_attention(p, dtype, c.ctx->stream); })) return rc;
       c.ctx->status_pending = true;
       *out = keep(&r, dtype, b, sq, hq, d);

@@ -65,6 +65,7 @@ struct DecoderAttention {
   int causal;
   const int2* doc_ranges;     // [b, ceil(sk / 128)] smallest and largest id of each 128 keys, the smallest with its sign bit
                               // set when some of them belong to no document; set with documents
+  float* sums;                // prompt_attention_scratch() bytes, or null where that is none
   StatusWords status;
 };
 constexpr int kDocBlock = 128;
@@ -99,6 +100,7 @@ cudaError_t launch_cache_attention(const DecoderAttention& p, int dtype, const C
 
 // Prompts of 16-bit operands (prompt_attn.cu).
 bool prompt_attention_usable(const DecoderAttention& p, int dtype);
+int64_t prompt_attention_scratch(const DecoderAttention& p, int dtype);
 cudaError_t launch_prompt_attention(const DecoderAttention& p, int dtype, cudaStream_t s);
 
 // ---- sample.cu ---------------------------------------------------------------------------------------------------

@@ -253,3 +253,43 @@ def test_attention_of_float32_prompts_adds_without_a_bias(bridge, buffers, d, sq
     p = p * ((d + 16) * 2.0 ** -23 * (np.abs(q) @ np.abs(k).swapaxes(-1, -2)) / np.sqrt(d) + 2.0 ** -21)
     err = p @ np.abs(v - 3.0) + p.sum(-1, keepdims=True) * np.abs(want - 3.0) + want * (2 * 2.0 ** -21 + 10 * 2.0 ** -23 + (2 * (sk // 64) + 18 + 2) * 2.0 ** -24)
     within(got, want, err)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq,rule", [(64, "plain"), (130, "plain"), (300, "ragged"), (64, "capped")])
+def test_attention_of_long_caches_adds_without_a_bias(bridge, buffers, dtype, d, sq, rule):
+    """Equal scores over 140000 values of one sign, whose mean is the result.  The tensor core adds with truncation: 16 keys at a
+    time, two steps of 2^-23 each (of the products' sum and of the accumulator), for at most 64 tiles of 128 keys, 2^-13 of the
+    mean in all; then come the half step of the result and a few of 32 bits.  Left to itself the sum loses 2^-10 of itself."""
+    sk = 140000
+    rules = dict(causal=False, softcap=30.0 if rule == "capped" else 0.0)
+    if rule == "ragged":
+        rules.update(lengths=[sk, 70001])
+    v = 3.0 + np.clip(normal(5, 2, 1, sk, d), -3, 3) / 4
+    got = attend(bridge, buffers, dtype, np.zeros((2, 2, sq, d), np.float32), normal(6, 2, 1, sk, d), v, **rules)
+    v = rounded(v, dtype)
+    want = np.stack([v[i, :, :n].mean(1) for i, n in enumerate(rules.get("lengths", [sk, sk]))])[:, :, None]
+    want = np.broadcast_to(want, got.shape)
+    within(got, want, want * (2.0 ** -13 + oracle.HALF[dtype] + 2.0 ** -20))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rule", ["causal", "rising", "documents", "rows that begin late"])
+def test_attention_of_prompts_over_long_caches(bridge, buffers, dtype, d, rule):
+    """Sums that go on in memory: over references that rise on the way, rows that see their first key there, and few tiles."""
+    b, sq, sk = 1, 140, 26000
+    q, k, v = normal(1, b, 2, sq, d), normal(2, b, 1, sk, d), normal(3, b, 1, sk, d)
+    rules = dict(starts=[sk - sq])
+    if rule == "rising":
+        q, k = np.abs(q), k * 0.1
+        k[:, :, :, 0] = np.linspace(-8, 8, sk)
+    if rule == "documents":
+        rules.update(documents=np.repeat([0, 1], [9000, 17000])[None].astype(np.int32), starts=[9000 - sq // 2])
+    if rule == "rows that begin late":
+        ids = np.zeros((b, sk), np.int32)
+        ids[:, 12000:] = 1
+        rules.update(documents=ids, causal=False, starts=[12000 - sq // 2])
+    got = attend(bridge, buffers, dtype, q, k, v, **rules)
+    within(got, *expected(dtype, q, k, v, **rules))
