@@ -51,11 +51,18 @@ CacheAttnPlan cache_attention_plan(const DecoderAttention& p, int dtype, int sm_
   // heads: 155 us in two parts each, 128 in six; one of 131077, 4 key heads of two row tiles: 94 us in 112 parts, 65 in the
   // 74 of one round).
   const int head = cache_attn::padded_head(p.d);
+  // Keys that a group of warps adds one after another.  The tensor core adds with truncation, which makes results of 16-bit
+  // operands smaller by some 10^-7 for every 16 keys: 10^-4 after 16384, a fifth of the half step of float16 (500000 keys in two
+  // groups lost 1.6 * 10^-3); bfloat16 stands eight times as many.  fp32 tiles are added in 32 bits.
+  const long long group_keys = dtype == BG_F16 ? 16384 : dtype == BG_BF16 ? 131072 : (long long)1 << 40;
+  const int groups = (plan.row_tiles == 4 && head <= 128) || head <= 64 ? 8 / plan.row_tiles : 4 / plan.row_tiles;
+  const long long least = p.sk <= groups * group_keys ? 1 : (p.sk + groups * group_keys - 1) / (groups * group_keys);
   const double slots = (plan.row_tiles == 1 && dtype != BG_F32 && head > 64 && head <= 128 ? 3.0 : 2.0) * sm_count;      // CTAs that run at once
   long long splits = 1, most = (p.sk + 511) / 512;
   if (most > 128) most = 128;
+  if (most < least) most = least;
   double best = 1e300;
-  for (long long s = 1; s <= most; ++s) {
+  for (long long s = least; s <= most; ++s) {
     const double keys = (double)p.sk / (double)s, cta = keys + 384.0, ctas = (double)(units * s);
     const double rounds = ceil(ctas / slots);
     double t = plan.row_tiles == 1 ? fmax(ctas * cta / slots, 0.75 * cta * rounds) : rounds * cta;

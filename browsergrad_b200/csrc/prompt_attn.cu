@@ -49,8 +49,8 @@ constexpr int kRows = 128, kKeys = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyLog2 = 8.0f;
 // Key tiles that are added in tensor memory before O goes to a sum in memory (LONG: caches that have more).  The tensor core adds
-// with truncation, which makes a result smaller by some 6 * 10^-8 for each addition, eight a tile: 3 * 10^-5 after 64 tiles, but
-// 6 * 10^-4 after 131072 keys, more than the half step of float16.  64 rows of 8 heads of 128 over 131072 keys: 2144 us without
+// with truncation, which makes a result smaller by some 10^-7 for each addition, eight a tile: 5 * 10^-5 after 64 tiles, but
+// 8 * 10^-4 after 131072 keys, more than the half step of float16.  64 rows of 8 heads of 128 over 131072 keys: 2144 us without
 // the sums in memory, 2212 with them; their code alone would cost plain prompts of heads of 64 a tenth (394 -> 430 us), hence
 // kernels of their own.
 constexpr int kFoldTiles = 64;

@@ -293,3 +293,17 @@ def test_attention_of_prompts_over_long_caches(bridge, buffers, dtype, d, rule):
         rules.update(documents=ids, causal=False, starts=[12000 - sq // 2])
     got = attend(bridge, buffers, dtype, q, k, v, **rules)
     within(got, *expected(dtype, q, k, v, **rules))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d,group,sq", [(64, 8, 4), (128, 1, 1), (128, 8, 4), (128, 1, 63), (256, 1, 63)])
+def test_attention_of_many_long_caches_adds_without_a_bias(bridge, buffers, dtype, d, group, sq):
+    """The same where so many sequences fill the device that none is split for speed.  A group of warps adds at most 16384 keys
+    (bfloat16 131072) in the tensor core, 16 at a time, two steps of 2^-23 each: 2^-12 of the mean, or 2^-9."""
+    b, sk = 296, 500000
+    q = np.zeros((b, group, sq, d), np.float32)
+    k, v = normal(6, 1, 1, sk, d), 3.0 + np.clip(normal(5, 1, 1, sk, d), -3, 3) / 4
+    views = [HeadView(buffers.put(x, dtype), (0, d, sk * d)) for x in (k, v)]
+    out = buffers.own(bridge.decoder_attention(buffers.put(q, dtype), *views, b, group, 1, sq, sk, d, dtype, causal=False))
+    want = np.broadcast_to(rounded(v, dtype).mean(2, keepdims=True), q.shape)
+    within(buffers.get(out, q.shape, dtype), want, want * ((2.0 ** -12 if dtype == "float16" else 2.0 ** -9) + oracle.HALF[dtype] + 2.0 ** -20))
