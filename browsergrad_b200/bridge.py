@@ -231,9 +231,9 @@ class CudaBridge:
                       top_p: float = 1.0, min_p: float = 0.0, temperatures: Optional[int] = None, top_ks: Optional[int] = None,
                       top_ps: Optional[int] = None, min_ps: Optional[int] = None, probabilities: Optional[int] = None,
                       out: Optional[int] = None) -> int:
-        """One token (int64 ``[n]``) per row of ``logits [n, vocab]`` from the random numbers ``uniforms`` (float32 ``[n]``
-        in [0, 1)); ``vocab`` is at most 2^20.  Temperature 0 is greedy.  The plural parameters are per-row buffers (float32, ``top_ks`` int32);
-        ``probabilities`` names a float32 ``[n]`` buffer for the tokens' chances."""
+        """One token (int64 ``[n]``) per row of ``logits [n, vocab]``, ``vocab`` at most 2^20, from the random numbers
+        ``uniforms`` (float32 ``[n]`` in [0, 1)).  Temperature 0 is greedy.  The plural parameters are per-row buffers (float32,
+        ``top_ks`` int32); ``probabilities`` names a float32 ``[n]`` buffer for the tokens' chances."""
         r = C.c_int64()
         sampling = _lib.Sampling(temperature, top_p, min_p, top_k, temperatures or 0, top_ks or 0, top_ps or 0, min_ps or 0)
         self._check(self._lib.bg_sample_tokens(self._ctx, logits, uniforms, n, vocab, self._dt(dtype), C.byref(sampling),

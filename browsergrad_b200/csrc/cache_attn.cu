@@ -45,11 +45,13 @@ CacheAttnPlan cache_attention_plan(const DecoderAttention& p, int dtype, int sm_
   // How many CTAs share the keys: the number estimated to take the least time, in keys that an SM slot works through.  A
   // CTA costs its keys and about 384 more (start, join of its groups, partial result), the kernel that joins the splits
   // about 700.  Sequences of equal length run in whole rounds of CTAs; with one row tile the memory is the bound, and three
-  // quarters of the slots draw nearly all of it (256 sets of 8192 keys of 128, bf16: 167 us in one part each, 175 in three;
-  // 64 sets of 2048: 35 in one, 21 in four).  Where lengths are given they are taken to differ: few CTAs then wait for the
-  // longest (a third more), three rounds of not too short ones even out (32 sequences of about 5000 of 8192 keys, 8 key
-  // heads: 155 us in two parts each, 128 in six; one of 131077, 4 key heads of two row tiles: 94 us in 112 parts, 65 in the
-  // 74 of one round).
+  // quarters of the slots draw nearly all of it (64 sets of 2048 keys of 128, bf16: 34 us in one part each, 20 in the four it
+  // takes; 256 sets of 2048: 50 in the one it takes, 57 in three; 256 of 8192: 177 in the three it takes, where one would be
+  // 166).  Where lengths are given they are taken to differ: few CTAs then wait for the longest (a third more), three rounds of
+  // not too short ones even out (32 sequences of about 5000 of 8192 keys, 8 key heads: 155 us in two parts each, 128 in six; one
+  // of 131077, 4 key heads of two row tiles: 89 us in 112 parts, 79 in 37, 65 in the 74 of one round).  Heads above 128 run one
+  // CTA an SM, and so do few rows of fp32 heads above 64; counting two there costs up to 8 % on the longest caches (131072 keys,
+  // 8 heads of 256, bf16: 219 us, with one 202) and gains as much on 8192 keys (24.0, with one 26.6).
   const int head = cache_attn::padded_head(p.d);
   // Keys that a group of warps adds one after another.  The tensor core adds with truncation, which makes results of 16-bit
   // operands smaller by some 10^-7 for every 16 keys: 10^-4 after 16384, a fifth of the half step of float16 (500000 keys in two

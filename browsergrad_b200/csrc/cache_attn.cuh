@@ -15,9 +15,10 @@
 // added to O in registers, because the tensor core's own accumulation truncates.  16-bit P is rounded to the operand
 // type, because the tensor core multiplies two operands of one type: each probability is off by at most 2^-8 (bf16) or 2^-11
 // (f16) of itself, the half step the result is rounded by too; f16 ones below 2^-28 of the largest by up to 2^-39 of it.
-// Measured: 32 x 8 key heads of 8192 keys of 128, bf16, 167 us = 6.4 TB/s; 131077 keys, 4 key heads of two row tiles, f16,
-// 65 us (41 us at the copy rate; 8 warps an SM wait for their own tile's products and exponentials, DRAM 57 % busy);
-// 64 x 12 heads of 2048 keys of 64, fp32, 130 us = 6.2 TB/s; fp32 prompts of heads of 128 (2 x 16 x 2048, causal) 42 TFLOP/s.
+// Measured: 32 x 8 key heads of 8192 keys of 128, bf16, 177 us = 6.1 TB/s in the three parts the plan takes (166 in one);
+// 131077 keys, 4 key heads of two row tiles, f16, 65 to 69 us on different machines (41 us at the copy rate; 8 warps an SM wait
+// for their own tile's products and exponentials, DRAM 59 % busy); 64 x 12 heads of 2048 keys of 64, fp32, 128 us = 6.3 TB/s;
+// fp32 prompts of heads of 128 (2 x 16 x 2048, causal) 42 TFLOP/s.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -21,9 +21,9 @@
 // Bound: 4 D flops a visible pair on the tensor pipe (1024 clocks a tile of 128 x 128 x 128) against one exponential a
 // pair on the MUFU (16 a clock: 1024 clocks).  A cap would add two more MUFU operations; within |s| <= cap, where scores
 // nearly always lie, tanh is an odd polynomial on the FMA pipe instead, two values an instruction.
-// Measured: 4 x 16 heads of 4096 keys of 128, bf16, 548 us = 1004 TFLOP/s, causal 862; 2 x 16 heads of 4099 keys of 128, f16,
-// prefix and cap, 272 us = 521 TFLOP/s of visible pairs (tensor pipe 26 %, FMA pipe 37 %, MUFU 25 %: the chain of a tile,
-// scores - maximum - cap - exponentials - P V, is what it waits for).  P handed over in two halves gained nothing (557 us).
+// Measured: 4 x 16 heads of 4096 keys of 128, bf16, 549 us = 1001 TFLOP/s, causal 865; 2 x 16 heads of 4099 keys of 128, f16,
+// prefix and cap, 274 us = 517 TFLOP/s of visible pairs (tensor pipe 27 %, FMA pipe 39 %, MUFU 25 %: the chain of a tile,
+// scores - maximum - cap - exponentials - P V, is what it waits for).  P handed over in two halves gained nothing.
 // No cluster multicast; every wait is clock-bounded.
 #include "serving.h"
 
@@ -665,7 +665,8 @@ int query_tiles(const DecoderAttention& p) {
   // One query tile a CTA and two CTAs an SM where there is little work behind a CTA's start, which the other then covers:
   // 32 x 128 tokens 18 us against 24, 16 x 512 33 against 35 (capped 45 against 49), packed documents of 400 in 4 x 2048
   // 46 against 49; from 2048 keys on two tiles that share their keys and take turns win (capped 99.5 us against 101.5,
-  // 16 heads of 4096 keys 683 against 773).
+  // 16 heads of 4096 keys 683 against 773).  Packed documents in 4 x 12 heads of 4096 tokens, one tile against two: of 100 tokens
+  // 71 us against 77, of 1024 91 against 98, of 2048 126 against 127, one of 4096 199 against 188.
   return p.documents || p.sk <= 1024 ? 1 : 2;
 }
 
@@ -675,7 +676,10 @@ bool prompt_attention_usable(const DecoderAttention& p, int dtype) {
   if (dtype == BG_F32) return prompt_attention32_usable(p);
   if ((dtype != BG_BF16 && dtype != BG_F16) || p.d > 128 || p.d % 8 || p.sk == 0 || !encode_fn()) return false;
   // Below 64 rows a head most of a 128-row tile would stand empty, and the key-split kernel reads each key once for the
-  // whole group.
+  // whole group: 63 rows there against 64 here, 8 x 12 heads of 64 over 1024 keys 28 us against 20, over 64 keys 10.9 against
+  // 11.7, 8 x 8 heads of 128 in groups of four over 1024 keys 44 against 25.  These kernels do not split the keys, so few query
+  // tiles over a long cache leave most SMs idle, and there the key-split kernel would be the faster one: 64 rows of 8 heads of
+  // 128 over 16384 keys 261 us against its 42 for 63 rows, over 131072 keys 2.2 ms against 185 us.
   if (p.sq < 64) return false;
   if (smem_bytes<128, 2>(p.sk) > 227 * 1024) return false;
   if ((long long)((p.sq + 127) / 128) * p.b * p.hq > 0x7fffffffll) return false;

@@ -7,9 +7,10 @@
 // Angles: t f_j reaches 10^6 radians and more, where 32 bits leave no fraction; the product is formed in 64 bits as turns
 // (f_j / 2 pi comes from the host), its whole part is taken off, and sine and cosine of the fraction are 32-bit.  The
 // rotation is done in 32 bits and rounded once to the stored type.
-// Eight CTAs an SM (32 registers a thread) hide the load latency: 32771 tokens of 32 heads of 128, bf16, 96 us = 5.6 TB/s; at 40
-// registers 104 us, with the next item fetched ahead 121 us.  Ragged prompts into a cache (6 x 1537 tokens, 32 + 8 + 8 heads of
-// 128, f16, interleaved pairs) 39 us = 5.3 TB/s, instruction issue 68 % busy.
+// Eight CTAs an SM (32 registers a thread) hide the load latency: 32771 tokens of 32 heads of 128, bf16, 96 to 108 us on different
+// machines = 5.0 to 5.6 TB/s; on the fastest of them 104 us at 40 registers and 121 with the next item fetched ahead.  Ragged
+// prompts into a cache (6 x 1537 tokens, 32 + 8 + 8 heads of 128, f16, interleaved pairs) 39 to 41 us = 5.1 to 5.3 TB/s,
+// instruction issue 68 % busy.
 #include "serving.h"
 
 #include <cuda_bf16.h>
